@@ -86,7 +86,8 @@ class use_library:
 def torch_acl_dtype(t):
     import torch
     return {torch.float32: ACL_FLOAT, torch.float16: ACL_FLOAT16, torch.bfloat16: ACL_BF16, torch.int8: ACL_INT8,
-            torch.uint8: ACL_UINT8, torch.int32: ACL_INT32, torch.int64: ACL_INT64}[t.dtype]
+            torch.uint8: ACL_UINT8, torch.int32: ACL_INT32, torch.int64: ACL_INT64, torch.float8_e4m3fn: ACL_FLOAT8_E4M3FN,
+            torch.float8_e5m2: ACL_FLOAT8_E5M2}[t.dtype]
 
 
 class AclTensor:
@@ -295,3 +296,119 @@ def cast(src, src_kind, dst_kind, n, **kw):
         dst = torch.empty(n, dtype=torch.uint8, device=src.device)
     call("aclnnCast", AclTensor(src, src_kind, (n,)), ctypes.c_int(dst_kind), AclTensor(dst, dst_kind, (n,)), **kw)
     return dst
+
+
+# ---------------------------------------------------------------- the expert layer: fp8 with a scale per 128 (aclnn_block_quant_moe.h)
+def _check(*tensors):
+    """The ABI takes dense tensors on one GPU; a view of anything else would be misread."""
+    dev = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda or not t.is_contiguous():
+            raise ValueError("the expert-layer operators take contiguous CUDA tensors")
+        if dev is not None and t.device != dev:
+            raise ValueError(f"tensors on {dev} and {t.device}")
+        dev = t.device
+
+
+def _opt(t):
+    return AclTensor(t) if t is not None else None
+
+
+def block_quant_fp8(x, row_block=1, dtype=None, **kw):
+    """x [..., D] f32/f16/bf16 -> (fp8 codes of x's shape, fp32 scales).  One scale per 128 columns of a row
+    ([..., ceil(D/128)]), or with row_block=128 per 128 x 128 block of the matrix x ([ceil(rows/128), ceil(D/128)])."""
+    import torch
+    _check(x)
+    q = torch.empty(x.shape, dtype=dtype or torch.float8_e4m3fn, device=x.device)
+    blocks = (x.shape[-1] + 127) // 128
+    if row_block == 1:
+        scale = torch.empty(x.shape[:-1] + (blocks,), dtype=torch.float32, device=x.device)
+    else:
+        rows = x.numel() // x.shape[-1] if x.shape[-1] else 0
+        scale = torch.empty(((rows + row_block - 1) // row_block, blocks), dtype=torch.float32, device=x.device)
+    call("aclnnB200BlockQuantFp8", AclTensor(x), ctypes.c_int64(row_block), AclTensor(q), AclTensor(scale), **kw)
+    return q, scale
+
+
+def swiglu_block_quant_fp8(x, dtype=None, **kw):
+    """x [..., 2D] f32/f16/bf16 -> (fp8 codes [..., D] of silu(x[..., :D]) * x[..., D:], fp32 scales [..., ceil(D/128)])."""
+    import torch
+    _check(x)
+    D = x.shape[-1] // 2
+    q = torch.empty(x.shape[:-1] + (D,), dtype=dtype or torch.float8_e4m3fn, device=x.device)
+    scale = torch.empty(x.shape[:-1] + ((D + 127) // 128,), dtype=torch.float32, device=x.device)
+    call("aclnnB200SwiGluBlockQuantFp8", AclTensor(x), AclTensor(q), AclTensor(scale), **kw)
+    return q, scale
+
+
+def block_quant_matmul(x, x_scale, w, w_scale, transposed=False, out_dtype=None, out=None, **kw):
+    """x fp8 [M,K] with x_scale [M, ceil(K/128)]; w fp8 [K,N] (transposed: [N,K]) with a scale per 128 x 128 block."""
+    import torch
+    if out is None:
+        out = torch.empty((x.shape[0], w.shape[0 if transposed else 1]), dtype=out_dtype or torch.bfloat16, device=x.device)
+    _check(x, x_scale, w, w_scale, out)
+    call("aclnnB200BlockQuantMatmul", AclTensor(x), AclTensor(x_scale), AclTensor(w), AclTensor(w_scale), ctypes.c_bool(transposed), AclTensor(out), **kw)
+    return out
+
+
+def block_quant_grouped_matmul(x, x_scale, w, w_scale, rows_per_expert, transposed=False, out_dtype=None, out=None, **kw):
+    """The same per expert: w [E,K,N] (or [E,N,K]), rows_per_expert int64 [E] on the device.  Rows of `out` behind the
+    last expert's are left as they were."""
+    import torch
+    if out is None:
+        out = torch.empty((x.shape[0], w.shape[1 if transposed else 2]), dtype=out_dtype or torch.bfloat16, device=x.device)
+    _check(x, x_scale, w, w_scale, rows_per_expert, out)
+    call("aclnnB200BlockQuantGroupedMatmul", AclTensor(x), AclTensor(x_scale), AclTensor(w), AclTensor(w_scale), AclTensor(rows_per_expert),
+         ctypes.c_bool(transposed), AclTensor(out), **kw)
+    return out
+
+
+def moe_token_permute(tokens, expert_ids, num_experts, scales=None, out=None, scales_out=None, **kw):
+    """tokens [T,H], expert_ids int32/int64 [T,k] -> (rows [T*k,H] sorted by expert, place int32 [T,k], rows per expert
+    int64 [num_experts][, scale rows [T*k,S]]).  Ids outside [0, num_experts) are dropped (place -1); the rows behind the
+    last one are left as they were in `out` / `scales_out`."""
+    import torch
+    T, k = expert_ids.shape
+    dev = tokens.device
+    if out is None:
+        out = torch.empty((T * k, tokens.shape[1]), dtype=tokens.dtype, device=dev)
+    if scales is not None and scales_out is None:
+        scales_out = torch.empty((out.shape[0], scales.shape[1]), dtype=torch.float32, device=dev)
+    place = torch.empty((T, k), dtype=torch.int32, device=dev)
+    counts = torch.empty((num_experts,), dtype=torch.int64, device=dev)
+    _check(tokens, expert_ids, scales, out, scales_out)
+    call("aclnnB200MoeTokenPermute", AclTensor(tokens), AclTensor(expert_ids), _opt(scales), AclTensor(out), _opt(scales_out), AclTensor(place),
+         AclTensor(counts), **kw)
+    return (out, place, counts) if scales is None else (out, place, counts, scales_out)
+
+
+def moe_token_permute_grad(grad_rows, place, **kw):
+    """The gradient of moe_token_permute's tokens: the sum of each token's rows of grad_rows."""
+    import torch
+    out = torch.empty((place.shape[0], grad_rows.shape[1]), dtype=grad_rows.dtype, device=grad_rows.device)
+    _check(grad_rows, place)
+    call("aclnnB200MoeTokenPermuteGrad", AclTensor(grad_rows), AclTensor(place), AclTensor(out), **kw)
+    return out
+
+
+def moe_token_unpermute(rows, place, probs=None, **kw):
+    """rows [R,H], place int32 [T,k], probs [T,k] -> out [T,H]: the weighted sum of each token's rows."""
+    import torch
+    out = torch.empty((place.shape[0], rows.shape[1]), dtype=rows.dtype, device=rows.device)
+    _check(rows, place, probs)
+    call("aclnnB200MoeTokenUnpermute", AclTensor(rows), AclTensor(place), _opt(probs), AclTensor(out), **kw)
+    return out
+
+
+def moe_token_unpermute_grad(grad_out, rows, place, probs, out=None, **kw):
+    """The gradients of moe_token_unpermute: (of rows, of probs).  Rows of `out` that no pair names are left as they were
+    (zeros where `out` is not given)."""
+    import torch
+    if out is None:
+        out = torch.zeros_like(rows)
+    dprobs = torch.empty_like(probs)
+    _check(grad_out, rows, place, probs, out)
+    call("aclnnB200MoeTokenUnpermuteGrad", AclTensor(grad_out), AclTensor(rows), AclTensor(place), AclTensor(probs), AclTensor(out), AclTensor(dprobs), **kw)
+    return out, dprobs

@@ -20,6 +20,11 @@ enum PlanOp : int {
     PLAN_SWIGLUQUANT, // SwiGLU fused with the per-token quantiser
     PLAN_MXQUANT,     // block-wise power-of-two-scale int8 quantiser
     PLAN_ADDRMSNORM,  // residual add + RMS norm (tail of the all-reduce matmuls)
+    PLAN_BLOCKQUANT,  // fp8 codes with one scale per 128 columns (rows of x, or rows of SwiGLU(x))
+    PLAN_BLOCKMM,     // block-scaled fp8 matmul, dense or per expert
+    PLAN_PERMUTE,     // tokens sorted by expert
+    PLAN_UNPERMUTE,   // weighted sum of a token's rows (and the gradient of the sort)
+    PLAN_UNPERMUTE_GRAD, // gradients of the weighted sum
     PLAN_WRAPPER,     // plan of a composite operator living in another library (payload + deleter below)
 };
 
@@ -43,6 +48,10 @@ struct aclOpExecutor {
     const aclTensor *pertoken = nullptr;
     aclTensor *out = nullptr;
     aclTensor *out2 = nullptr;            // second output (per-token scales of the dynamic quantiser)
+    aclTensor *out3 = nullptr, *out4 = nullptr;   // PLAN_PERMUTE: place, rows per expert
+    int64_t experts = 0;                  // PLAN_BLOCKMM: E (0 = dense); PLAN_PERMUTE: E
+    int64_t topk = 0, width = 0;          // PLAN_PERMUTE / PLAN_UNPERMUTE*: choices per token; scales per row
+    bool swiglu = false;                  // PLAN_BLOCKQUANT
     int64_t batch = 1, m = 0, n = 0, k = 0;
     int64_t group = 0;          // rows of K per antiquant scale row (K for per-channel)
     bool b_transposed = false;  // weight stored [N,K]

@@ -1,0 +1,270 @@
+// Operator layer of the expert-layer operators (aclnn_block_quant_moe.h): phase 1 checks and plans, phase 2 launches.
+#include <cstdint>
+#include <new>
+
+#include "aclnnop/aclnn_block_quant_moe.h"
+#include "executor.h"
+#include "kernels.h"
+#include "plan_utils.h"
+
+using namespace qmm;
+
+namespace {
+
+bool is_fp8(aclDataType t) { return t == ACL_FLOAT8_E4M3FN || t == ACL_FLOAT8_E5M2; }
+
+// No negative size, dense, ND, and few enough elements for 64-bit byte offsets.
+bool sane(const aclTensor *t) {
+    double n = 1;
+    for (auto d : t->viewDims) {
+        if (d < 0) return false;
+        n *= d > 0 ? (double)d : 1.0;
+    }
+    return n < 1e17 && t->format == ACL_FORMAT_ND && t->offset >= 0 && dense(t);
+}
+int64_t bytes_of(const aclTensor *t) { return t->numel() * (int64_t)dtype_size(t->dtype); }
+char *ptr_of(const aclTensor *t) { return t && t->data ? (char *)t->data + t->offset * (int64_t)dtype_size(t->dtype) : nullptr; }
+
+// 161001 for a missing pointer, 161002 for an output that overlaps another tensor of the call.
+aclnnStatus check_pointers(std::initializer_list<const aclTensor *> in, std::initializer_list<const aclTensor *> out) {
+    for (auto &list : {in, out})
+        for (const aclTensor *t : list)
+            if (t && bytes_of(t) > 0 && !t->data) return ACLNN_ERR_PARAM_NULLPTR;
+    auto meet = [](const aclTensor *a, const aclTensor *b) {
+        if (!a || !b || bytes_of(a) == 0 || bytes_of(b) == 0) return false;
+        const char *pa = ptr_of(a), *pb = ptr_of(b);
+        return pa < pb + bytes_of(b) && pb < pa + bytes_of(a);
+    };
+    for (auto o = out.begin(); o != out.end(); ++o) {
+        for (const aclTensor *i : in) if (meet(*o, i)) return ACLNN_ERR_PARAM_INVALID;
+        for (auto q = o + 1; q != out.end(); ++q) if (meet(*o, *q)) return ACLNN_ERR_PARAM_INVALID;
+    }
+    return ACLNN_SUCCESS;
+}
+
+aclnnStatus finish(aclOpExecutor *e, uint64_t *ws, aclOpExecutor **ex) {
+    *ws = e->ws_bytes;
+    *ex = e;
+    return ACLNN_SUCCESS;
+}
+
+aclnnStatus block_quant_plan(const aclTensor *x, int64_t row_block, bool swiglu, aclTensor *out, aclTensor *scale, uint64_t *ws, aclOpExecutor **ex) {
+    if (!x || !out || !scale || !ws || !ex) return ACLNN_ERR_PARAM_NULLPTR;
+    if (!is_float_act(x->dtype) || !is_fp8(out->dtype) || scale->dtype != ACL_FLOAT) return ACLNN_ERR_PARAM_INVALID;
+    if (row_block != 1 && row_block != 128) return ACLNN_ERR_PARAM_INVALID;
+    if (x->rank() < 1 || x->rank() != out->rank() || !sane(x) || !sane(out) || !sane(scale)) return ACLNN_ERR_PARAM_INVALID;
+    const int64_t D = out->viewDims.back();
+    if (x->viewDims.back() != (swiglu ? 2 * D : D)) return ACLNN_ERR_PARAM_INVALID;
+    int64_t rows = 1;
+    for (int i = 0; i + 1 < x->rank(); ++i) {
+        if (x->viewDims[i] != out->viewDims[i]) return ACLNN_ERR_PARAM_INVALID;
+        rows *= x->viewDims[i];
+    }
+    if (D == 0) rows = 0;
+    if (scale->numel() != (rows + row_block - 1) / row_block * ((D + 127) / 128)) return ACLNN_ERR_PARAM_INVALID;
+    auto *e = new (std::nothrow) aclOpExecutor();
+    if (!e) return ACLNN_ERR_RUNTIME_ERROR;
+    e->op = PLAN_BLOCKQUANT; e->a = x; e->out = out; e->out2 = scale; e->m = rows; e->k = D; e->group = row_block; e->swiglu = swiglu;
+    return finish(e, ws, ex);
+}
+
+aclnnStatus block_mm_plan(const aclTensor *x, const aclTensor *xs, const aclTensor *w, const aclTensor *wscale, const aclTensor *groups, bool grouped,
+                          bool nk, aclTensor *out, uint64_t *ws, aclOpExecutor **ex) {
+    if (!x || !xs || !w || !wscale || (grouped && !groups) || !out || !ws || !ex) return ACLNN_ERR_PARAM_NULLPTR;
+    if (!is_fp8(x->dtype) || !is_fp8(w->dtype) || xs->dtype != ACL_FLOAT || wscale->dtype != ACL_FLOAT || !is_float_act(out->dtype))
+        return ACLNN_ERR_PARAM_INVALID;
+    const int lead = grouped ? 1 : 0;
+    if (x->rank() != 2 || w->rank() != 2 + lead || wscale->rank() != 2 + lead || out->rank() != 2) return ACLNN_ERR_PARAM_INVALID;
+    for (const aclTensor *t : {x, xs, w, wscale, (const aclTensor *)out}) if (!sane(t)) return ACLNN_ERR_PARAM_INVALID;
+    const int64_t M = x->viewDims[0], K = x->viewDims[1], N = w->viewDims[lead + (nk ? 0 : 1)];
+    const int64_t E = grouped ? w->viewDims[0] : 0, kb = (K + 127) / 128, nb = (N + 127) / 128;
+    if (K < 1 || N < 1 || w->viewDims[lead + (nk ? 1 : 0)] != K || !shape_is(out, {M, N}) || !shape_is(xs, {M, kb})) return ACLNN_ERR_PARAM_INVALID;
+    if (M > (1LL << 30) || N > (1LL << 30) || K > (1LL << 30)) return ACLNN_ERR_PARAM_INVALID;
+    if (wscale->viewDims[lead] != (nk ? nb : kb) || wscale->viewDims[lead + 1] != (nk ? kb : nb)) return ACLNN_ERR_PARAM_INVALID;
+    if (grouped) {
+        if (E < 1 || E > BLOCK_MM_MAX_EXPERTS || wscale->viewDims[0] != E) return ACLNN_ERR_PARAM_INVALID;
+        if (groups->dtype != ACL_INT64 || !shape_is(groups, {E}) || !sane(groups)) return ACLNN_ERR_PARAM_INVALID;
+    }
+    auto *e = new (std::nothrow) aclOpExecutor();
+    if (!e) return ACLNN_ERR_RUNTIME_ERROR;
+    e->op = PLAN_BLOCKMM; e->a = x; e->b = w; e->scale = xs; e->scale2 = wscale; e->pertoken = groups; e->out = out;
+    e->m = M; e->n = N; e->k = K; e->experts = E; e->b_transposed = nk;
+    return finish(e, ws, ex);
+}
+
+aclnnStatus permute_plan(const aclTensor *tokens, const aclTensor *ids, const aclTensor *scales, aclTensor *rows, aclTensor *scales_out,
+                         aclTensor *place, aclTensor *counts, uint64_t *ws, aclOpExecutor **ex) {
+    if (!tokens || !ids || !rows || !place || !counts || !ws || !ex || (!scales) != (!scales_out)) return ACLNN_ERR_PARAM_NULLPTR;
+    for (const aclTensor *t : {tokens, ids, (const aclTensor *)rows, (const aclTensor *)place, (const aclTensor *)counts})
+        if (!sane(t)) return ACLNN_ERR_PARAM_INVALID;
+    if (!is_float_act(tokens->dtype) && !is_fp8(tokens->dtype) && tokens->dtype != ACL_INT8) return ACLNN_ERR_PARAM_INVALID;
+    if (rows->dtype != tokens->dtype || (ids->dtype != ACL_INT32 && ids->dtype != ACL_INT64) || place->dtype != ACL_INT32 || counts->dtype != ACL_INT64)
+        return ACLNN_ERR_PARAM_INVALID;
+    if (tokens->rank() != 2 || rows->rank() != 2 || ids->rank() != 2 || counts->rank() != 1) return ACLNN_ERR_PARAM_INVALID;
+    const int64_t T = tokens->viewDims[0], H = tokens->viewDims[1], k = ids->viewDims[1], E = counts->viewDims[0], R = rows->viewDims[0];
+    if (ids->viewDims[0] != T || !shape_is(place, {T, k}) || rows->viewDims[1] != H || k < 1 || k > MOE_MAX_TOPK || E < 1 || E > MOE_MAX_EXPERTS)
+        return ACLNN_ERR_PARAM_INVALID;
+    if (T > (1LL << 30) / k || R < T * k) return ACLNN_ERR_PARAM_INVALID;
+    if (scales) {
+        if (!sane(scales) || !sane(scales_out) || scales->dtype != ACL_FLOAT || scales_out->dtype != ACL_FLOAT || scales->rank() != 2 ||
+            scales->viewDims[0] != T || !shape_is(scales_out, {R, scales->viewDims[1]})) return ACLNN_ERR_PARAM_INVALID;
+    }
+    auto *e = new (std::nothrow) aclOpExecutor();
+    if (!e) return ACLNN_ERR_RUNTIME_ERROR;
+    e->op = PLAN_PERMUTE; e->a = tokens; e->b = ids; e->scale = scales; e->out = rows; e->out2 = scales_out; e->out3 = place; e->out4 = counts;
+    e->m = T; e->k = H; e->topk = k; e->experts = E; e->width = scales ? scales->viewDims[1] : 0;
+    return finish(e, ws, ex);
+}
+
+aclnnStatus unpermute_plan(const aclTensor *rows, const aclTensor *place, const aclTensor *probs, aclTensor *out, uint64_t *ws, aclOpExecutor **ex) {
+    if (!rows || !place || !out || !ws || !ex) return ACLNN_ERR_PARAM_NULLPTR;
+    if (!sane(rows) || !sane(place) || !sane(out) || (probs && !sane(probs))) return ACLNN_ERR_PARAM_INVALID;
+    if (!is_float_act(rows->dtype) || out->dtype != rows->dtype || place->dtype != ACL_INT32 || (probs && !is_float_act(probs->dtype)))
+        return ACLNN_ERR_PARAM_INVALID;
+    if (rows->rank() != 2 || out->rank() != 2 || place->rank() != 2) return ACLNN_ERR_PARAM_INVALID;
+    const int64_t T = out->viewDims[0], H = out->viewDims[1], k = place->viewDims[1];
+    if (rows->viewDims[1] != H || place->viewDims[0] != T || k < 1 || k > MOE_MAX_TOPK || T > (1LL << 30) / k || rows->viewDims[0] > 0x7fffffffLL)
+        return ACLNN_ERR_PARAM_INVALID;
+    if (probs && !shape_is(probs, {T, k})) return ACLNN_ERR_PARAM_INVALID;
+    auto *e = new (std::nothrow) aclOpExecutor();
+    if (!e) return ACLNN_ERR_RUNTIME_ERROR;
+    e->op = PLAN_UNPERMUTE; e->a = rows; e->b = place; e->scale = probs; e->out = out;
+    e->m = T; e->k = H; e->n = rows->viewDims[0]; e->topk = k;
+    return finish(e, ws, ex);
+}
+
+aclnnStatus unpermute_grad_plan(const aclTensor *dout, const aclTensor *rows, const aclTensor *place, const aclTensor *probs, aclTensor *drows,
+                                aclTensor *dprobs, uint64_t *ws, aclOpExecutor **ex) {
+    if (!dout || !rows || !place || !probs || !drows || !dprobs || !ws || !ex) return ACLNN_ERR_PARAM_NULLPTR;
+    for (const aclTensor *t : {dout, rows, place, probs, (const aclTensor *)drows, (const aclTensor *)dprobs})
+        if (!sane(t)) return ACLNN_ERR_PARAM_INVALID;
+    if (!is_float_act(rows->dtype) || dout->dtype != rows->dtype || drows->dtype != rows->dtype || place->dtype != ACL_INT32 ||
+        !is_float_act(probs->dtype) || dprobs->dtype != probs->dtype) return ACLNN_ERR_PARAM_INVALID;
+    if (rows->rank() != 2 || dout->rank() != 2 || place->rank() != 2 || drows->viewDims != rows->viewDims) return ACLNN_ERR_PARAM_INVALID;
+    const int64_t T = dout->viewDims[0], H = dout->viewDims[1], k = place->viewDims[1];
+    if (rows->viewDims[1] != H || place->viewDims[0] != T || k < 1 || k > MOE_MAX_TOPK || T > (1LL << 30) / k || rows->viewDims[0] > 0x7fffffffLL)
+        return ACLNN_ERR_PARAM_INVALID;
+    if (!shape_is(probs, {T, k}) || !shape_is(dprobs, {T, k})) return ACLNN_ERR_PARAM_INVALID;
+    auto *e = new (std::nothrow) aclOpExecutor();
+    if (!e) return ACLNN_ERR_RUNTIME_ERROR;
+    e->op = PLAN_UNPERMUTE_GRAD; e->a = dout; e->b = rows; e->pertoken = place; e->scale = probs; e->out = drows; e->out2 = dprobs;
+    e->m = T; e->k = H; e->n = rows->viewDims[0]; e->topk = k;
+    return finish(e, ws, ex);
+}
+
+aclnnStatus launch_plan(const aclOpExecutor *e, void *ws, uint64_t ws_bytes, cudaStream_t s) {
+    if (e->ws_bytes > 0 && (!ws || ws_bytes < e->ws_bytes)) return ACLNN_ERR_PARAM_INVALID;
+    cudaError_t err = cudaSuccess;
+    aclnnStatus st;
+    switch (e->op) {
+        case PLAN_BLOCKQUANT:
+            if ((st = check_pointers({e->a}, {e->out, e->out2}))) return st;
+            err = launch_block_quant(ptr_of(e->a), elem_type(e->a->dtype), e->group, e->swiglu, (uint8_t *)ptr_of(e->out), elem_type(e->out->dtype),
+                                     (float *)ptr_of(e->out2), e->m, e->k, s);
+            break;
+        case PLAN_BLOCKMM: {
+            if ((st = check_pointers({e->a, e->b, e->scale, e->scale2, e->pertoken}, {e->out}))) return st;
+            BlockMmArgs p;
+            p.x = (const uint8_t *)ptr_of(e->a); p.w = (const uint8_t *)ptr_of(e->b);
+            p.xs = (const float *)ptr_of(e->scale); p.ws = (const float *)ptr_of(e->scale2);
+            p.group_rows = (const int64_t *)ptr_of(e->pertoken); p.out = ptr_of(e->out);
+            p.x_type = elem_type(e->a->dtype); p.w_type = elem_type(e->b->dtype); p.out_type = elem_type(e->out->dtype);
+            p.M = e->m; p.N = e->n; p.K = e->k; p.experts = e->experts; p.w_nk = e->b_transposed;
+            if (p.M > 0) err = launch_block_mm(p, s);
+            break;
+        }
+        case PLAN_PERMUTE: {
+            if ((st = check_pointers({e->a, e->b, e->scale}, {e->out, e->out2, e->out3, e->out4}))) return st;
+            PermuteArgs p;
+            p.tokens = ptr_of(e->a); p.ids = ptr_of(e->b); p.scales = (const float *)ptr_of(e->scale);
+            p.rows = ptr_of(e->out); p.scales_out = (float *)ptr_of(e->out2); p.place = (int32_t *)ptr_of(e->out3); p.counts = (int64_t *)ptr_of(e->out4);
+            p.T = e->m; p.k = e->topk; p.E = e->experts; p.row_bytes = e->k * (int64_t)dtype_size(e->a->dtype); p.S = e->width;
+            p.ids64 = e->b->dtype == ACL_INT64;
+            err = launch_moe_permute(p, s);
+            break;
+        }
+        case PLAN_UNPERMUTE:
+            if ((st = check_pointers({e->a, e->b, e->scale}, {e->out}))) return st;
+            err = launch_moe_unpermute(ptr_of(e->a), elem_type(e->a->dtype), (const int32_t *)ptr_of(e->b), ptr_of(e->scale),
+                                       e->scale ? elem_type(e->scale->dtype) : (int)ET_NONE, ptr_of(e->out), e->m, e->topk, e->n, e->k, s);
+            break;
+        case PLAN_UNPERMUTE_GRAD:
+            if ((st = check_pointers({e->a, e->b, e->pertoken, e->scale}, {e->out, e->out2}))) return st;
+            err = launch_moe_unpermute_grad(ptr_of(e->a), ptr_of(e->b), elem_type(e->a->dtype), (const int32_t *)ptr_of(e->pertoken), ptr_of(e->scale),
+                                            elem_type(e->scale->dtype), ptr_of(e->out), ptr_of(e->out2), e->m, e->topk, e->n, e->k, s);
+            break;
+        default: return ACLNN_ERR_PARAM_INVALID;
+    }
+    if (err != cudaSuccess) {
+        fprintf(stderr, "[b200-qmm] launch failed: %s\n", cudaGetErrorString(err));
+        return ACLNN_ERR_RUNTIME_ERROR;
+    }
+    return ACLNN_SUCCESS;
+}
+
+aclnnStatus run_plan(PlanOp op, void *ws, uint64_t ws_bytes, aclOpExecutor *e, aclrtStream stream) {
+    if (!e) return ACLNN_ERR_PARAM_NULLPTR;
+    aclnnStatus st;
+    if (e->op != op) {
+        st = ACLNN_ERR_PARAM_INVALID;   // a plan of another operator
+    } else if (op == PLAN_BLOCKMM && latched_status_of_current_device()) {
+        fprintf(stderr, "[b200-qmm] refusing to launch: an earlier kernel on this device gave up a bounded wait; call "
+                        "aclnnB200ResetDeviceStatus() once the cause is understood\n");
+        st = ACLNN_ERR_RUNTIME_ERROR;
+    } else {
+        st = launch_plan(e, ws, ws_bytes, (cudaStream_t)stream);
+    }
+    delete e;
+    return st;
+}
+
+}  // namespace
+
+extern "C" {
+
+#define RUN_EXPERT(NAME, OP) \
+    aclnnStatus NAME(void *ws, uint64_t wsz, aclOpExecutor *e, aclrtStream s) { return run_plan(OP, ws, wsz, e, s); }
+
+aclnnStatus aclnnB200BlockQuantFp8GetWorkspaceSize(const aclTensor *x, int64_t rowBlockSize, aclTensor *out, aclTensor *scaleOut, uint64_t *ws,
+                                                   aclOpExecutor **ex) {
+    return block_quant_plan(x, rowBlockSize, false, out, scaleOut, ws, ex);
+}
+RUN_EXPERT(aclnnB200BlockQuantFp8, PLAN_BLOCKQUANT)
+aclnnStatus aclnnB200SwiGluBlockQuantFp8GetWorkspaceSize(const aclTensor *x, aclTensor *out, aclTensor *scaleOut, uint64_t *ws, aclOpExecutor **ex) {
+    return block_quant_plan(x, 1, true, out, scaleOut, ws, ex);
+}
+RUN_EXPERT(aclnnB200SwiGluBlockQuantFp8, PLAN_BLOCKQUANT)
+
+aclnnStatus aclnnB200BlockQuantMatmulGetWorkspaceSize(const aclTensor *x, const aclTensor *xScale, const aclTensor *weight,
+        const aclTensor *weightScale, bool transposeWeight, aclTensor *out, uint64_t *ws, aclOpExecutor **ex) {
+    return block_mm_plan(x, xScale, weight, weightScale, nullptr, false, transposeWeight, out, ws, ex);
+}
+RUN_EXPERT(aclnnB200BlockQuantMatmul, PLAN_BLOCKMM)
+aclnnStatus aclnnB200BlockQuantGroupedMatmulGetWorkspaceSize(const aclTensor *x, const aclTensor *xScale, const aclTensor *weight,
+        const aclTensor *weightScale, const aclTensor *groupRows, bool transposeWeight, aclTensor *out, uint64_t *ws, aclOpExecutor **ex) {
+    return block_mm_plan(x, xScale, weight, weightScale, groupRows, true, transposeWeight, out, ws, ex);
+}
+RUN_EXPERT(aclnnB200BlockQuantGroupedMatmul, PLAN_BLOCKMM)
+
+aclnnStatus aclnnB200MoeTokenPermuteGetWorkspaceSize(const aclTensor *tokens, const aclTensor *expertIds, const aclTensor *scalesOptional,
+        aclTensor *rowsOut, aclTensor *scalesOutOptional, aclTensor *place, aclTensor *rowsPerExpert, uint64_t *ws, aclOpExecutor **ex) {
+    return permute_plan(tokens, expertIds, scalesOptional, rowsOut, scalesOutOptional, place, rowsPerExpert, ws, ex);
+}
+RUN_EXPERT(aclnnB200MoeTokenPermute, PLAN_PERMUTE)
+aclnnStatus aclnnB200MoeTokenPermuteGradGetWorkspaceSize(const aclTensor *gradRows, const aclTensor *place, aclTensor *gradTokens, uint64_t *ws,
+                                                         aclOpExecutor **ex) {
+    return unpermute_plan(gradRows, place, nullptr, gradTokens, ws, ex);
+}
+RUN_EXPERT(aclnnB200MoeTokenPermuteGrad, PLAN_UNPERMUTE)
+aclnnStatus aclnnB200MoeTokenUnpermuteGetWorkspaceSize(const aclTensor *rows, const aclTensor *place, const aclTensor *probsOptional, aclTensor *out,
+                                                       uint64_t *ws, aclOpExecutor **ex) {
+    return unpermute_plan(rows, place, probsOptional, out, ws, ex);
+}
+RUN_EXPERT(aclnnB200MoeTokenUnpermute, PLAN_UNPERMUTE)
+aclnnStatus aclnnB200MoeTokenUnpermuteGradGetWorkspaceSize(const aclTensor *gradOut, const aclTensor *rows, const aclTensor *place,
+        const aclTensor *probs, aclTensor *gradRows, aclTensor *gradProbs, uint64_t *ws, aclOpExecutor **ex) {
+    return unpermute_grad_plan(gradOut, rows, place, probs, gradRows, gradProbs, ws, ex);
+}
+RUN_EXPERT(aclnnB200MoeTokenUnpermuteGrad, PLAN_UNPERMUTE_GRAD)
+
+}  // extern "C"

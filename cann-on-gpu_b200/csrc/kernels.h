@@ -137,6 +137,42 @@ bool wq_mma_gather_consumed();
 cudaError_t launch_rows_bf16_to_scaled_f16(const void *x, void *xh, float *rowscale, int64_t M, int64_t K, cudaStream_t s);
 void tc_reserve_sms(int n);   // the calling thread's dense-kernel plans leave n SMs free (0 = none)
 
+// fp8 codes with one fp32 scale per 128 columns (block_quant.cu).  row_block 1 or 128; swiglu: x is [rows][2 D] (row_block 1).
+cudaError_t launch_block_quant(const void *x, int x_type, int64_t row_block, bool swiglu, uint8_t *q, int q_type, float *scale_out,
+                               int64_t rows, int64_t D, cudaStream_t s);
+
+// Block-scaled fp8 matmul (block_mm.cu), dense (experts = 0) or per expert.
+struct BlockMmArgs {
+    const uint8_t *x = nullptr, *w = nullptr;
+    const float *xs = nullptr, *ws = nullptr;      // [M][kb]; [kb][nb] or, with w_nk, [nb][kb] (per expert)
+    const int64_t *group_rows = nullptr;           // [experts], on the device
+    void *out = nullptr;
+    int x_type = ET_NONE, w_type = ET_NONE, out_type = ET_NONE;
+    int64_t M = 0, N = 0, K = 0, experts = 0;
+    bool w_nk = false;                             // weight [N,K] instead of [K,N]
+};
+constexpr int BLOCK_MM_MAX_EXPERTS = 1024;
+cudaError_t launch_block_mm(const BlockMmArgs &p, cudaStream_t s);
+
+// Tokens sorted by expert and back (moe_permute.cu).
+constexpr int MOE_MAX_EXPERTS = 1024, MOE_MAX_TOPK = 64;
+struct PermuteArgs {
+    const void *tokens = nullptr, *ids = nullptr;
+    const float *scales = nullptr;
+    void *rows = nullptr;
+    float *scales_out = nullptr;
+    int32_t *place = nullptr;
+    int64_t *counts = nullptr;
+    int64_t T = 0, k = 0, E = 0, row_bytes = 0, S = 0;
+    bool ids64 = false;
+};
+cudaError_t launch_moe_permute(const PermuteArgs &p, cudaStream_t s);
+// out[t] = sum_j probs[t,j] * rows[place[t,j]]; probs may be null (weights of one).
+cudaError_t launch_moe_unpermute(const void *rows, int type, const int32_t *place, const void *probs, int probs_type, void *out,
+                                 int64_t T, int64_t k, int64_t R, int64_t H, cudaStream_t s);
+cudaError_t launch_moe_unpermute_grad(const void *dout, const void *rows, int type, const int32_t *place, const void *probs, int probs_type,
+                                      void *drows, void *dprobs, int64_t T, int64_t k, int64_t R, int64_t H, cudaStream_t s);
+
 // Host-side tally of kernels this library has launched (diagnostics for benchmarks).
 void count_launch(int n = 1);
 uint64_t launch_count();

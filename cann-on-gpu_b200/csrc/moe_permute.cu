@@ -1,0 +1,327 @@
+// Tokens sorted by expert and back, with the gradients of both.
+//
+// place[t,j] is the row of pair (token t, choice j) in the order by (expert, t, j); pairs whose expert is not in [0,E) have
+// place -1 and no row.  Everything is a stable counting sort and row copies: no atomics whose order could show, sums in
+// fp32 in the order of j.
+#include "device_utils.cuh"
+
+namespace qmm {
+namespace {
+
+__device__ __forceinline__ int expert_of(const void *ids, bool ids64, int64_t i, int E) {
+    if (ids64) {
+        const int64_t e = __ldg((const long long *)ids + i);
+        return e >= 0 && e < E ? (int)e : -1;
+    }
+    const int e = __ldg((const int *)ids + i);
+    return e >= 0 && e < E ? e : -1;
+}
+
+// ---- the sort: one cluster of 8 CTAs, no workspace ------------------------------------------------
+// The pairs are cut into 8 x 32 contiguous warp shares.  Pass 1 counts experts per warp (lanes of one expert find each
+// other with match_any), then each expert's counts are summed over the warps before, the CTAs before (distributed shared
+// memory) and the experts before; pass 2 walks the shares again and hands out places in order.
+constexpr int SORT_CTAS = 8, SORT_WARPS = 32;
+
+__device__ __forceinline__ void cluster_arrive() { __syncwarp(); asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ int ld_remote(const int *local, int cta) {
+    uint32_t a = (uint32_t)__cvta_generic_to_shared(local), r;
+    int v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(cta));
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(r) : "memory");
+    return v;
+}
+
+__global__ void __cluster_dims__(SORT_CTAS, 1, 1) __launch_bounds__(SORT_WARPS * 32)
+moe_sort_kernel(const void *ids, bool ids64, int32_t *place, int64_t *counts, int64_t N, int E) {
+    extern __shared__ int hist[];                 // [SORT_WARPS][E], then [E] totals of the CTA
+    __shared__ int scan[32];
+    int *cta_total = hist + SORT_WARPS * E;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, cta = blockIdx.x;
+    int *mine = hist + warp * E;
+    for (int i = lane; i < E; i += 32) mine[i] = 0;
+    __syncwarp();
+    const int64_t share = (N + SORT_CTAS * SORT_WARPS * 32 - 1) / (SORT_CTAS * SORT_WARPS * 32) * 32;
+    const int64_t lo = (int64_t)(cta * SORT_WARPS + warp) * share, hi = lo + share < N ? lo + share : N;
+    for (int64_t i0 = lo; i0 < hi; i0 += 32) {
+        const int64_t i = i0 + lane;
+        const int e = i < hi ? expert_of(ids, ids64, i, E) : -1;
+        const unsigned same = __match_any_sync(0xffffffffu, e);
+        if (e >= 0 && (same & ((1u << lane) - 1)) == 0) mine[e] += __popc(same);
+        __syncwarp();
+    }
+    __syncthreads();
+    if (tid < E) {
+        int run = 0;
+        for (int w = 0; w < SORT_WARPS; ++w) {
+            const int c = hist[w * E + tid];
+            hist[w * E + tid] = run;
+            run += c;
+        }
+        cta_total[tid] = run;
+    }
+    cluster_arrive();
+    cluster_wait();
+    int before = 0, total = 0;
+    if (tid < E) {
+#pragma unroll
+        for (int c = 0; c < SORT_CTAS; ++c) {
+            const int v = ld_remote(cta_total + tid, c);
+            before += c < cta ? v : 0;
+            total += v;
+        }
+    }
+    cluster_arrive();                             // this CTA has read the others' totals; they may not exit before that
+    int incl = total;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += v;
+    }
+    if (lane == 31) scan[warp] = incl;
+    __syncthreads();
+    int base = incl - total + before;
+    for (int w = 0; w < warp; ++w) base += scan[w];
+    if (tid < E) {
+        for (int w = 0; w < SORT_WARPS; ++w) hist[w * E + tid] += base;
+        if (cta == 0) counts[tid] = total;
+    }
+    __syncthreads();
+    for (int64_t i0 = lo; i0 < hi; i0 += 32) {
+        const int64_t i = i0 + lane;
+        const int e = i < hi ? expert_of(ids, ids64, i, E) : -1;
+        const unsigned same = __match_any_sync(0xffffffffu, e);
+        const unsigned below = same & ((1u << lane) - 1);
+        const int at = e >= 0 ? mine[e] + __popc(below) : -1;
+        __syncwarp();
+        if (e >= 0 && below == 0) mine[e] += __popc(same);
+        __syncwarp();
+        if (i < hi) place[i] = at;
+    }
+    cluster_wait();
+}
+
+// ---- rows to their places ------------------------------------------------------------------------
+// A warp takes 4 x 32 units of one token's row, reads them once and writes them to each of the token's rows.
+template <typename U>
+__global__ void __launch_bounds__(256) moe_scatter_kernel(const U *tokens, const float *scales, const int32_t *place, U *rows, float *scales_out,
+                                                          int64_t T, int k, int64_t units, int64_t S, int64_t segs) {
+    const int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    const int64_t t = w / segs, seg = w - t * segs;
+    if (t >= T) return;
+    const int32_t p0 = lane < k ? __ldg(place + t * k + lane) : -1, p1 = lane + 32 < k ? __ldg(place + t * k + lane + 32) : -1;
+    U v[4];
+    const int64_t u0 = seg * 128 + lane;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (u0 + 32 * i < units) v[i] = __ldg(tokens + t * units + u0 + 32 * i);
+    for (int j = 0; j < k; ++j) {
+        const int64_t r = __shfl_sync(0xffffffffu, j < 32 ? p0 : p1, j & 31);
+        if (r < 0) continue;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (u0 + 32 * i < units) rows[r * units + u0 + 32 * i] = v[i];
+    }
+    if (seg == 0) {
+        for (int64_t c = lane; c - lane < S; c += 32) {
+            const float sc = c < S ? __ldg(scales + t * S + c) : 0.f;
+            for (int j = 0; j < k; ++j) {
+                const int64_t r = __shfl_sync(0xffffffffu, j < 32 ? p0 : p1, j & 31);
+                if (r >= 0 && c < S) scales_out[r * S + c] = sc;
+            }
+        }
+    }
+}
+
+// ---- 16 bytes of a row as floats -----------------------------------------------------------------
+// EPV elements per lane: consecutive with VEC (one 16-byte access), else 32 apart (lane-contiguous scalar accesses).
+template <int T> constexpr int epv() { return T == ET_F32 ? 4 : 8; }
+template <int T, bool VEC> struct RowPiece {
+    static constexpr int N = epv<T>();
+    static __device__ __forceinline__ int64_t col(int64_t seg, int lane, int i) {
+        return VEC ? seg * (32 * N) + lane * N + i : seg * (32 * N) + i * 32 + lane;
+    }
+    static __device__ __forceinline__ void load(const void *p, int64_t row, int64_t H, int64_t seg, int lane, float (&f)[N]) {
+        if constexpr (VEC) {
+            if (col(seg, lane, 0) >= H) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) f[i] = 0.f;
+                return;
+            }
+            const uint4 v = __ldg(reinterpret_cast<const uint4 *>((const char *)p + (row * H + col(seg, lane, 0)) * (T == ET_F32 ? 4 : 2)));
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (T == ET_F32) f[i] = __uint_as_float(w[i]);
+                else if constexpr (T == ET_BF16) { f[2 * i] = __uint_as_float(w[i] << 16); f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u); }
+                else { f[2 * i] = __half2float(__ushort_as_half((unsigned short)(w[i] & 0xFFFFu))); f[2 * i + 1] = __half2float(__ushort_as_half((unsigned short)(w[i] >> 16))); }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) f[i] = col(seg, lane, i) < H ? load_as_float(p, T, row * H + col(seg, lane, i)) : 0.f;
+        }
+    }
+    static __device__ __forceinline__ void store(void *p, int64_t row, int64_t H, int64_t seg, int lane, const float (&f)[N]) {
+        if constexpr (VEC) {
+            if (col(seg, lane, 0) >= H) return;
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (T == ET_F32) w[i] = __float_as_uint(f[i]);
+                else if constexpr (T == ET_BF16) { __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]); w[i] = *reinterpret_cast<uint32_t *>(&h); }
+                else { __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]); w[i] = *reinterpret_cast<uint32_t *>(&h); }
+            }
+            *reinterpret_cast<uint4 *>((char *)p + (row * H + col(seg, lane, 0)) * (T == ET_F32 ? 4 : 2)) = make_uint4(w[0], w[1], w[2], w[3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (col(seg, lane, i) < H) store_from_float(p, T, row * H + col(seg, lane, i), f[i]);
+        }
+    }
+};
+
+// ---- weighted sum of a token's rows --------------------------------------------------------------
+// A warp takes 32 x 16 bytes of one token's output and sums them over the token's rows.
+template <int T, bool VEC>
+__global__ void __launch_bounds__(256) moe_gather_kernel(const void *rows, const int32_t *place, const void *probs, int probs_type, void *out,
+                                                         int64_t n_tokens, int k, int64_t R, int64_t H, int64_t segs) {
+    using P = RowPiece<T, VEC>;
+    const int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    const int64_t t = w / segs, seg = w - t * segs;
+    if (t >= n_tokens) return;
+    float acc[P::N] = {};
+    for (int j0 = 0; j0 < k; j0 += 32) {
+        const bool has = j0 + lane < k;
+        const int32_t pl = has ? __ldg(place + t * k + j0 + lane) : -1;
+        const float pr = has && probs ? load_as_float(probs, probs_type, t * k + j0 + lane) : 1.f;
+        const int n = k - j0 < 32 ? k - j0 : 32;
+        for (int j = 0; j < n; ++j) {
+            const int32_t r = __shfl_sync(0xffffffffu, pl, j);
+            const float f = __shfl_sync(0xffffffffu, pr, j);
+            if (r < 0 || r >= R) continue;
+            float v[P::N];
+            P::load(rows, r, H, seg, lane, v);
+#pragma unroll
+            for (int i = 0; i < P::N; ++i) acc[i] += f * v[i];
+        }
+    }
+    P::store(out, t, H, seg, lane, acc);
+}
+
+// ---- gradients of the weighted sum ---------------------------------------------------------------
+// A CTA per token: its warps share the row's segments, write probs * gradOut into each of the token's rows and sum
+// <gradOut, row>; the warps' sums meet in shared memory in a fixed order.
+constexpr int GRAD_J = 8;
+template <int T, bool VEC>
+__global__ void __launch_bounds__(256) moe_gather_grad_kernel(const void *dout, const void *rows, const int32_t *place, const void *probs, int probs_type,
+                                                              void *drows, void *dprobs, int k, int64_t R, int64_t H, int64_t segs) {
+    using P = RowPiece<T, VEC>;
+    __shared__ float part[8][GRAD_J];
+    const int64_t t = blockIdx.x;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    for (int j0 = 0; j0 < k; j0 += GRAD_J) {
+        float dot[GRAD_J], pr[GRAD_J];
+        int32_t pl[GRAD_J];
+#pragma unroll
+        for (int j = 0; j < GRAD_J; ++j) {
+            dot[j] = 0.f;
+            const bool has = j0 + j < k;
+            pl[j] = has ? __ldg(place + t * k + j0 + j) : -1;
+            if (pl[j] >= R) pl[j] = -1;
+            pr[j] = has ? load_as_float(probs, probs_type, t * k + j0 + j) : 0.f;
+        }
+        for (int64_t seg = warp; seg < segs; seg += warps) {
+            float g[P::N];
+            P::load(dout, t, H, seg, lane, g);
+#pragma unroll
+            for (int j = 0; j < GRAD_J; ++j) {
+                if (pl[j] < 0) continue;
+                float v[P::N], o[P::N];
+                P::load(rows, pl[j], H, seg, lane, v);
+#pragma unroll
+                for (int i = 0; i < P::N; ++i) { dot[j] += g[i] * v[i]; o[i] = pr[j] * g[i]; }
+                P::store(drows, pl[j], H, seg, lane, o);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < GRAD_J; ++j) {
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], o);
+            if (lane == 0) part[warp][j] = dot[j];
+        }
+        __syncthreads();
+        if (threadIdx.x < GRAD_J && j0 + threadIdx.x < k) {
+            float s = 0.f;
+            for (int w = 0; w < warps; ++w) s += part[w][threadIdx.x];
+            store_from_float(dprobs, probs_type, t * k + j0 + threadIdx.x, s);
+        }
+        __syncthreads();
+    }
+}
+
+bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+template <typename U> cudaError_t launch_scatter(const PermuteArgs &p, cudaStream_t s) {
+    const int64_t units = p.row_bytes / (int64_t)sizeof(U), segs = units > 128 ? (units + 127) / 128 : 1, warps = p.T * segs;
+    if ((warps + 7) / 8 > 0x7fffffffLL) return cudaErrorInvalidValue;
+    moe_scatter_kernel<U><<<(unsigned)((warps + 7) / 8), 256, 0, s>>>((const U *)p.tokens, p.scales, p.place, (U *)p.rows, p.scales_out, p.T, (int)p.k,
+                                                                     units, p.S, segs);
+    count_launch();
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_moe_permute(const PermuteArgs &p, cudaStream_t s) {
+    const size_t smem = (size_t)(SORT_WARPS + 1) * p.E * 4;
+    cudaError_t e = cudaFuncSetAttribute(moe_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (SORT_WARPS + 1) * MOE_MAX_EXPERTS * 4);
+    if (e != cudaSuccess) return e;
+    moe_sort_kernel<<<SORT_CTAS, SORT_WARPS * 32, smem, s>>>(p.ids, p.ids64, p.place, p.counts, p.T * p.k, (int)p.E);
+    count_launch();
+    e = cudaGetLastError();
+    if (e != cudaSuccess || p.T == 0 || (p.row_bytes == 0 && p.S == 0)) return e;
+    const uintptr_t all = reinterpret_cast<uintptr_t>(p.tokens) | reinterpret_cast<uintptr_t>(p.rows) | (uintptr_t)p.row_bytes;
+    if (all % 16 == 0) return launch_scatter<uint4>(p, s);
+    if (all % 4 == 0) return launch_scatter<uint32_t>(p, s);
+    if (all % 2 == 0) return launch_scatter<uint16_t>(p, s);
+    return launch_scatter<uint8_t>(p, s);
+}
+
+cudaError_t launch_moe_unpermute(const void *rows, int type, const int32_t *place, const void *probs, int probs_type, void *out,
+                                 int64_t T, int64_t k, int64_t R, int64_t H, cudaStream_t s) {
+    if (T <= 0 || H <= 0) return cudaSuccess;
+    const int per = type == ET_F32 ? 4 : 8;
+    const bool vec = H % per == 0 && aligned16(rows) && aligned16(out);
+    const int64_t segs = (H + 32 * per - 1) / (32 * per), ctas = (T * segs + 7) / 8;
+    if (ctas > 0x7fffffffLL) return cudaErrorInvalidValue;
+#define MG(TT) do { if (vec) moe_gather_kernel<TT, true><<<(unsigned)ctas, 256, 0, s>>>(rows, place, probs, probs_type, out, T, (int)k, R, H, segs); \
+                    else moe_gather_kernel<TT, false><<<(unsigned)ctas, 256, 0, s>>>(rows, place, probs, probs_type, out, T, (int)k, R, H, segs); } while (0)
+    if (type == ET_BF16) MG(ET_BF16);
+    else if (type == ET_F16) MG(ET_F16);
+    else MG(ET_F32);
+#undef MG
+    count_launch();
+    return cudaGetLastError();
+}
+
+cudaError_t launch_moe_unpermute_grad(const void *dout, const void *rows, int type, const int32_t *place, const void *probs, int probs_type,
+                                      void *drows, void *dprobs, int64_t T, int64_t k, int64_t R, int64_t H, cudaStream_t s) {
+    if (T <= 0) return cudaSuccess;
+    const int per = type == ET_F32 ? 4 : 8;
+    const bool vec = H % per == 0 && aligned16(dout) && aligned16(rows) && aligned16(drows);
+    const int64_t segs = (H + 32 * per - 1) / (32 * per);
+    const unsigned threads = (unsigned)(segs < 1 ? 32 : (segs < 8 ? 32 * segs : 256));
+#define MGG(TT) do { if (vec) moe_gather_grad_kernel<TT, true><<<(unsigned)T, threads, 0, s>>>(dout, rows, place, probs, probs_type, drows, dprobs, (int)k, R, H, segs); \
+                     else moe_gather_grad_kernel<TT, false><<<(unsigned)T, threads, 0, s>>>(dout, rows, place, probs, probs_type, drows, dprobs, (int)k, R, H, segs); } while (0)
+    if (type == ET_BF16) MGG(ET_BF16);
+    else if (type == ET_F16) MGG(ET_F16);
+    else MGG(ET_F32);
+#undef MGG
+    count_launch();
+    return cudaGetLastError();
+}
+
+}  // namespace qmm

@@ -13,28 +13,11 @@
 #include "aclnnop/aclnn_quant_matmul.h"
 #include "executor.h"
 #include "kernels.h"
+#include "plan_utils.h"
 
 using namespace qmm;
 
 namespace {
-
-int elem_type(aclDataType t) {
-    switch (t) {
-        case ACL_FLOAT: return ET_F32;
-        case ACL_FLOAT16: return ET_F16;
-        case ACL_BF16: return ET_BF16;
-        case ACL_INT8: return ET_I8;
-        case ACL_UINT8: return ET_U8;
-        case ACL_INT4: return ET_I4;
-        case ACL_INT32: return ET_I32;
-        case ACL_FLOAT8_E4M3FN: return ET_E4M3;
-        case ACL_FLOAT8_E5M2: return ET_E5M2;
-        case ACL_FLOAT4_E2M1: return ET_E2M1;
-        case ACL_FLOAT8_E8M0: return ET_E8M0;
-        default: return ET_NONE;
-    }
-}
-bool is_float_act(aclDataType t) { return t == ACL_FLOAT || t == ACL_FLOAT16 || t == ACL_BF16; }
 
 // Path override for A/B measurements: B200_QMM_PATH=generic|gemv|tc (unset = automatic).
 int forced_path() {
@@ -48,12 +31,6 @@ int forced_path() {
 bool debug_on() {
     static const bool on = getenv("B200_QMM_DBG") != nullptr;
     return on;
-}
-
-const void *data_of(const aclTensor *t) {
-    if (!t || !t->data) return nullptr;
-    // Sub-byte tensors cannot carry an odd element offset; validated in phase 1.
-    return (const char *)t->data + t->offset * (int64_t)elem_bits(elem_type(t->dtype)) / 8;
 }
 
 // MatmulArgs of a plan with the tensors' current data pointers.
@@ -142,11 +119,15 @@ void choose_path(aclOpExecutor *e, uint64_t *ws) {
 // application is expected to find out why before it goes on (aclnnB200ResetDeviceStatus() clears it).
 std::atomic<uint32_t> g_latched_status[64];
 
+}  // namespace
+namespace qmm {
 uint32_t latched_status_of_current_device() {
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
     return g_latched_status[dev].load(std::memory_order_relaxed);
 }
+}  // namespace qmm
+namespace {
 
 aclnnStatus run_matmul(void *ws, uint64_t ws_bytes, aclOpExecutor *e, aclrtStream stream) {
     if (!e) return ACLNN_ERR_PARAM_NULLPTR;
@@ -187,14 +168,6 @@ aclnnStatus run_matmul(void *ws, uint64_t ws_bytes, aclOpExecutor *e, aclrtStrea
     delete e;
     return st;
 }
-
-bool shape_is(const aclTensor *t, std::initializer_list<int64_t> dims) {
-    if (t->viewDims.size() != dims.size()) return false;
-    size_t i = 0;
-    for (auto d : dims) if (t->viewDims[i++] != d) return false;
-    return true;
-}
-bool dense(const aclTensor *t) { return t->contiguous(); }
 
 // ---- weight-only quantized matmul ------------------------------------------------------------------
 aclnnStatus wqbmm_plan(const aclTensor *x, const aclTensor *weight, const aclTensor *scale, const aclTensor *offset,

@@ -1,0 +1,108 @@
+/*
+ * aclnn_block_quant_moe.h -- a mixture-of-experts layer with 8-bit floating-point weights and activations,
+ * behind the same two-phase operator ABI as aclnn_quant_matmul.h: quantise, sort tokens by expert, multiply
+ * (dense or per expert), and return to token order, with the gradients of the two re-orderings.
+ *
+ * None of these names exists in the reference, hence the aclnnB200 prefix.  A layer runs
+ *
+ *     aclnnB200BlockQuantFp8        x [T,H]            -> q, s
+ *     aclnnB200MoeTokenPermute      q, s, expert ids   -> rows sorted by expert, place, rows per expert
+ *     aclnnB200BlockQuantGroupedMatmul (gate and up)   -> h [R,2F]
+ *     aclnnB200SwiGluBlockQuantFp8  h                  -> q, s
+ *     aclnnB200BlockQuantGroupedMatmul (down)          -> y [R,H]
+ *     aclnnB200MoeTokenUnpermute    y, place, probs    -> out [T,H]
+ *
+ * without a host round trip: the rows per expert stay on the device.
+ *
+ * Common rules.  All tensors are dense (contiguous) in ACL_FORMAT_ND; outputs overlap neither inputs nor each other
+ * (161002 at phase 2).  Sizes of zero are allowed where a batch may be empty.  Phase 1 returns 161001 for null arguments and
+ * 161002 for unsupported types or shapes; phase 2 returns 161001 for a null data pointer, 161002 for a workspace that
+ * is too small or a plan of another operator, 361001 for a launch error, and consumes the executor.  Calls keep no state: results do not
+ * depend on earlier calls, and the same inputs give the same bits.
+ */
+#ifndef B200_ACLNN_BLOCK_QUANT_MOE_H
+#define B200_ACLNN_BLOCK_QUANT_MOE_H
+
+#include <stdbool.h>
+
+#include "aclnnop/aclnn_quant_matmul.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+/* ---- Block quantiser to fp8 ----------------------------------------------------------------------
+ * x [..., D] (ACL_FLOAT, ACL_FLOAT16, ACL_BF16) seen as rows of D; one fp32 scale per block of rowBlockSize rows x 128
+ * columns (the last block of a row, and the last rows, may be shorter): scale = max(max|x| / top, 2^-126) with top = 448
+ * (ACL_FLOAT8_E4M3FN) or 57344 (ACL_FLOAT8_E5M2), 1 for a block of zeros; out = fp8(x * (1 / scale)), rounded to nearest
+ * even, saturating.  A NaN stays a NaN and does not enter the maximum; a block with an infinity has an infinite scale.
+ * rowBlockSize: 1 (activations: scaleOut [rows, ceil(D/128)]) or 128 (weights: scaleOut [ceil(rows/128), ceil(D/128)]);
+ * scaleOut is checked by its element count. */
+ACL_FUNC_VISIBILITY aclnnStatus aclnnB200BlockQuantFp8GetWorkspaceSize(const aclTensor *x, int64_t rowBlockSize, aclTensor *out,
+    aclTensor *scaleOut, uint64_t *workspaceSize, aclOpExecutor **executor);
+B200_ACLNN_RUN(aclnnB200BlockQuantFp8)
+
+/* SwiGLU in front of the same (rowBlockSize 1): x [..., 2 D] holds a = x[..., :D] and b = x[..., D:]; the values
+ * quantised are a / (1 + exp(-a)) * b in fp32. */
+ACL_FUNC_VISIBILITY aclnnStatus aclnnB200SwiGluBlockQuantFp8GetWorkspaceSize(const aclTensor *x, aclTensor *out, aclTensor *scaleOut,
+    uint64_t *workspaceSize, aclOpExecutor **executor);
+B200_ACLNN_RUN(aclnnB200SwiGluBlockQuantFp8)
+
+/* ---- Block-scaled fp8 matmul ---------------------------------------------------------------------
+ * out[m,n] = sum over blocks b of 128 k's:  xScale[m,b] * weightScale[b,n/128] * sum_{k in b} x[m,k] * weight[k,n]
+ * x [M,K] and weight of ACL_FLOAT8_E4M3FN or ACL_FLOAT8_E5M2 (they may differ), xScale ACL_FLOAT [M, ceil(K/128)].
+ * transposeWeight false: weight [K,N], weightScale ACL_FLOAT [ceil(K/128), ceil(N/128)]; true: weight [N,K],
+ * weightScale [ceil(N/128), ceil(K/128)].  out [M,N]: ACL_BF16, ACL_FLOAT16 or ACL_FLOAT.  Products and sums are fp32,
+ * with one rounding to out's type.  K >= 1, N >= 1, M >= 0. */
+ACL_FUNC_VISIBILITY aclnnStatus aclnnB200BlockQuantMatmulGetWorkspaceSize(const aclTensor *x, const aclTensor *xScale,
+    const aclTensor *weight, const aclTensor *weightScale, bool transposeWeight, aclTensor *out,
+    uint64_t *workspaceSize, aclOpExecutor **executor);
+B200_ACLNN_RUN(aclnnB200BlockQuantMatmul)
+
+/* The same per expert: weight [E,K,N] (or [E,N,K]) with weightScale [E,...], E <= 1024; groupRows ACL_INT64 [E] ON THE
+ * DEVICE holds the rows of each expert, which follow one another in x from row 0 (as aclnnB200MoeTokenPermute leaves
+ * them).  Rows of out behind the last expert's are left as they were.  A negative count counts as 0, and counts that
+ * run past M are cut there. */
+ACL_FUNC_VISIBILITY aclnnStatus aclnnB200BlockQuantGroupedMatmulGetWorkspaceSize(const aclTensor *x, const aclTensor *xScale,
+    const aclTensor *weight, const aclTensor *weightScale, const aclTensor *groupRows, bool transposeWeight, aclTensor *out,
+    uint64_t *workspaceSize, aclOpExecutor **executor);
+B200_ACLNN_RUN(aclnnB200BlockQuantGroupedMatmul)
+
+/* ---- Tokens sorted by expert ---------------------------------------------------------------------
+ * expertIds ACL_INT32 or ACL_INT64 [T,k] (k <= 64): the experts of each token.  The T*k (token, choice) pairs are sorted by
+ * expert, pairs of one expert staying in order (token, then choice); pair (t, j) takes row place[t,j] of rowsOut, which becomes
+ * tokens[t].  An id outside [0,E) drops its pair: place = -1.  E = number of elements of rowsPerExpert (1 to 1024).
+ * tokens [T,H] and rowsOut [R,H], R >= T*k: one type of ACL_FLOAT, ACL_FLOAT16, ACL_BF16, ACL_INT8, ACL_FLOAT8_E4M3FN,
+ * ACL_FLOAT8_E5M2.  Optional scales ACL_FLOAT [T,S] travel along into scalesOut [R,S] (both or neither).
+ * place ACL_INT32 [T,k]; rowsPerExpert ACL_INT64 [E].  Rows behind the last sorted one are left as they were. */
+ACL_FUNC_VISIBILITY aclnnStatus aclnnB200MoeTokenPermuteGetWorkspaceSize(const aclTensor *tokens, const aclTensor *expertIds,
+    const aclTensor *scalesOptional, aclTensor *rowsOut, aclTensor *scalesOutOptional, aclTensor *place, aclTensor *rowsPerExpert,
+    uint64_t *workspaceSize, aclOpExecutor **executor);
+B200_ACLNN_RUN(aclnnB200MoeTokenPermute)
+
+/* Its gradient: gradTokens[t] = sum_j gradRows[place[t,j]], summed in fp32 in the order of j, rounded once.
+ * gradRows [R,H] and gradTokens [T,H] of one type (ACL_FLOAT, ACL_FLOAT16, ACL_BF16).  Here and below a place outside
+ * [0,R) stands for no row. */
+ACL_FUNC_VISIBILITY aclnnStatus aclnnB200MoeTokenPermuteGradGetWorkspaceSize(const aclTensor *gradRows, const aclTensor *place,
+    aclTensor *gradTokens, uint64_t *workspaceSize, aclOpExecutor **executor);
+B200_ACLNN_RUN(aclnnB200MoeTokenPermuteGrad)
+
+/* ---- And back ------------------------------------------------------------------------------------
+ * out[t] = sum_j probs[t,j] * rows[place[t,j]] in fp32 in the order of j, rounded once; probs [T,k] (ACL_FLOAT,
+ * ACL_FLOAT16 or ACL_BF16) or NULL for weights of one.  A token without rows gets zeros. */
+ACL_FUNC_VISIBILITY aclnnStatus aclnnB200MoeTokenUnpermuteGetWorkspaceSize(const aclTensor *rows, const aclTensor *place,
+    const aclTensor *probsOptional, aclTensor *out, uint64_t *workspaceSize, aclOpExecutor **executor);
+B200_ACLNN_RUN(aclnnB200MoeTokenUnpermute)
+
+/* Its gradients: gradRows[place[t,j]] = probs[t,j] * gradOut[t]; gradProbs[t,j] = <gradOut[t], rows[place[t,j]]>
+ * (fp32 sums, 0 for a pair without a row), of probs' type.  Rows that no pair names are left as they were.  No row may
+ * be named by two pairs (aclnnB200MoeTokenPermute names none twice): of two, either one's product may be left. */
+ACL_FUNC_VISIBILITY aclnnStatus aclnnB200MoeTokenUnpermuteGradGetWorkspaceSize(const aclTensor *gradOut, const aclTensor *rows,
+    const aclTensor *place, const aclTensor *probs, aclTensor *gradRows, aclTensor *gradProbs,
+    uint64_t *workspaceSize, aclOpExecutor **executor);
+B200_ACLNN_RUN(aclnnB200MoeTokenUnpermuteGrad)
+
+#ifdef __cplusplus
+}
+#endif
+#endif

@@ -1,6 +1,9 @@
 // Block-scaled fp8 matmul, dense or per expert:
 //
 //   out[m,n] = sum_b xs[m,b] * ws[b,n/128] * ( sum_{k in block b} x[m,k] * w[k,n] ),   b = blocks of 128 k's
+//
+// The bounds-checked kernel for what the tensor-core kernel (block_mm_tc.cu) does not take: rows that are not a multiple of
+// 16 bytes, or operands off a 16-byte boundary.
 #include "device_utils.cuh"
 
 namespace qmm {
@@ -131,6 +134,8 @@ cudaError_t launch_simple(const BlockMmArgs &p, cudaStream_t s) {
 
 }  // namespace
 
-cudaError_t launch_block_mm(const BlockMmArgs &p, cudaStream_t s) { return launch_simple(p, s); }
+cudaError_t launch_block_mm(const BlockMmArgs &p, cudaStream_t s) {
+    return block_mm_tc_supported(p) ? launch_block_mm_tc(p, s) : launch_simple(p, s);
+}
 
 }  // namespace qmm

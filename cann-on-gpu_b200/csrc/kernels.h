@@ -153,6 +153,11 @@ struct BlockMmArgs {
 };
 constexpr int BLOCK_MM_MAX_EXPERTS = 1024;
 cudaError_t launch_block_mm(const BlockMmArgs &p, cudaStream_t s);
+// Its tensor-core form (block_mm_tc.cu).
+bool block_mm_tc_supported(const BlockMmArgs &p);
+cudaError_t launch_block_mm_tc(const BlockMmArgs &p, cudaStream_t s);
+unsigned int block_mm_device_status();
+void block_mm_device_status_reset();
 
 // Tokens sorted by expert and back (moe_permute.cu).
 constexpr int MOE_MAX_EXPERTS = 1024, MOE_MAX_TOPK = 64;

@@ -7,6 +7,7 @@ if the library is missing, `load()` raises.
 import ctypes
 import os
 import subprocess
+import threading
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libascendcl.so")
@@ -299,28 +300,100 @@ def cast(src, src_kind, dst_kind, n, **kw):
 
 
 # ---------------------------------------------------------------- the expert layer: fp8 with a scale per 128 (aclnn_block_quant_moe.h)
-def _check(*tensors):
-    """The ABI takes dense tensors on one GPU; a view of anything else would be misread."""
-    dev = None
-    for t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda or not t.is_contiguous():
-            raise ValueError("the expert-layer operators take contiguous CUDA tensors")
-        if dev is not None and t.device != dev:
-            raise ValueError(f"tensors on {dev} and {t.device}")
-        dev = t.device
+class _Call:
+    """One operator at one set of shapes and types: its aclTensor handles and prepared phase arguments.  A handle is
+    metadata only: every call points it at its own tensors first (aclSetRawTensorAddr), so nothing of a call's data is kept."""
+
+    def __init__(self, lib, name, args):
+        import torch
+        self.lib, self.handles = lib, []
+        self.phase1, self.phase2 = getattr(lib, name + "GetWorkspaceSize"), getattr(lib, name)
+        self.set_addr = lib.aclSetRawTensorAddr
+        self.set_addr.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
+        self.ws, self.ex = ctypes.c_uint64(0), ctypes.c_void_p(0)
+        self.ws_ptr, self.ws_size, self.stream = ctypes.c_void_p(0), ctypes.c_uint64(0), ctypes.c_void_p(0)
+        self.args = []
+        for a in args:
+            if isinstance(a, torch.Tensor):
+                dims = (ctypes.c_int64 * max(1, a.dim()))(*a.shape)
+                h = lib.aclCreateTensor(dims, a.dim(), torch_acl_dtype(a), None, 0, ACL_FORMAT_ND, dims, a.dim(), None)
+                if not h:
+                    raise RuntimeError("aclCreateTensor failed")
+                self.handles.append(h)
+                self.args.append(ctypes.c_void_p(h))
+            else:
+                self.args.append(None if a is None else (ctypes.c_bool(a) if isinstance(a, bool) else ctypes.c_int64(a)))
+        self.args += [ctypes.byref(self.ws), ctypes.byref(self.ex)]
+
+    def __del__(self):
+        try:
+            for h in self.handles:
+                self.lib.aclDestroyTensor(ctypes.c_void_p(h))
+        except Exception:
+            pass
 
 
-def _opt(t):
-    return AclTensor(t) if t is not None else None
+class _Calls(threading.local):   # a set of handles serves one call at a time: each thread has its own
+    MOST = 256
+
+    def __init__(self):
+        self.known = {}
+
+
+_calls = _Calls()
+
+
+def _run(name, *args, stream=None, return_status=False):
+    """The two phases of `name` on torch tensors, None, integers and truth values in phase 1's order, on the tensors'
+    device and torch's current stream there (or `stream`).  A workspace, where one is needed, is the call's own."""
+    import torch
+    T = torch.Tensor
+    lib = load()
+    dev, tensors, key = None, [], [name, id(lib)]
+    for a in args:
+        if isinstance(a, T):
+            # the ABI takes dense tensors on one GPU; a view of anything else would be misread
+            i = a.get_device()
+            if i < 0 or not a.is_contiguous():
+                raise ValueError("the expert-layer operators take contiguous CUDA tensors")
+            if i != dev:
+                if dev is not None:
+                    raise ValueError(f"tensors on devices {dev} and {i}")
+                dev = i
+            tensors.append(a)
+            key.append(a.shape)
+            key.append(a.dtype)
+        else:
+            key.append(a)
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return _run(name, *args, stream=stream, return_status=return_status)
+    key, known = tuple(key), _calls.known
+    c = known.get(key)
+    if c is None:
+        if len(known) >= _calls.MOST:
+            known.clear()
+        c = known[key] = _Call(lib, name, args)
+    set_addr = c.set_addr
+    for h, t in zip(c.handles, tensors):
+        set_addr(h, t.data_ptr())
+    st = c.phase1(*c.args)
+    if st == ACLNN_SUCCESS:
+        need = c.ws.value
+        ws = torch.empty(need, dtype=torch.uint8, device=tensors[0].device) if need else None
+        c.ws_ptr.value, c.ws_size.value = ws.data_ptr() if need else None, need
+        c.stream.value = torch.cuda.current_stream(dev).cuda_stream if stream is None else stream
+        st = c.phase2(c.ws_ptr, c.ws_size, c.ex, c.stream)
+    if return_status:
+        return st
+    if st != ACLNN_SUCCESS:
+        raise RuntimeError(f"{name} -> {st}")
 
 
 def block_quant_fp8(x, row_block=1, dtype=None, **kw):
     """x [..., D] f32/f16/bf16 -> (fp8 codes of x's shape, fp32 scales).  One scale per 128 columns of a row
     ([..., ceil(D/128)]), or with row_block=128 per 128 x 128 block of the matrix x ([ceil(rows/128), ceil(D/128)])."""
     import torch
-    _check(x)
     q = torch.empty(x.shape, dtype=dtype or torch.float8_e4m3fn, device=x.device)
     blocks = (x.shape[-1] + 127) // 128
     if row_block == 1:
@@ -328,18 +401,17 @@ def block_quant_fp8(x, row_block=1, dtype=None, **kw):
     else:
         rows = x.numel() // x.shape[-1] if x.shape[-1] else 0
         scale = torch.empty(((rows + row_block - 1) // row_block, blocks), dtype=torch.float32, device=x.device)
-    call("aclnnB200BlockQuantFp8", AclTensor(x), ctypes.c_int64(row_block), AclTensor(q), AclTensor(scale), **kw)
+    _run("aclnnB200BlockQuantFp8", x, row_block, q, scale, **kw)
     return q, scale
 
 
 def swiglu_block_quant_fp8(x, dtype=None, **kw):
     """x [..., 2D] f32/f16/bf16 -> (fp8 codes [..., D] of silu(x[..., :D]) * x[..., D:], fp32 scales [..., ceil(D/128)])."""
     import torch
-    _check(x)
     D = x.shape[-1] // 2
     q = torch.empty(x.shape[:-1] + (D,), dtype=dtype or torch.float8_e4m3fn, device=x.device)
     scale = torch.empty(x.shape[:-1] + ((D + 127) // 128,), dtype=torch.float32, device=x.device)
-    call("aclnnB200SwiGluBlockQuantFp8", AclTensor(x), AclTensor(q), AclTensor(scale), **kw)
+    _run("aclnnB200SwiGluBlockQuantFp8", x, q, scale, **kw)
     return q, scale
 
 
@@ -348,8 +420,7 @@ def block_quant_matmul(x, x_scale, w, w_scale, transposed=False, out_dtype=None,
     import torch
     if out is None:
         out = torch.empty((x.shape[0], w.shape[0 if transposed else 1]), dtype=out_dtype or torch.bfloat16, device=x.device)
-    _check(x, x_scale, w, w_scale, out)
-    call("aclnnB200BlockQuantMatmul", AclTensor(x), AclTensor(x_scale), AclTensor(w), AclTensor(w_scale), ctypes.c_bool(transposed), AclTensor(out), **kw)
+    _run("aclnnB200BlockQuantMatmul", x, x_scale, w, w_scale, bool(transposed), out, **kw)
     return out
 
 
@@ -359,9 +430,8 @@ def block_quant_grouped_matmul(x, x_scale, w, w_scale, rows_per_expert, transpos
     import torch
     if out is None:
         out = torch.empty((x.shape[0], w.shape[1 if transposed else 2]), dtype=out_dtype or torch.bfloat16, device=x.device)
-    _check(x, x_scale, w, w_scale, rows_per_expert, out)
-    call("aclnnB200BlockQuantGroupedMatmul", AclTensor(x), AclTensor(x_scale), AclTensor(w), AclTensor(w_scale), AclTensor(rows_per_expert),
-         ctypes.c_bool(transposed), AclTensor(out), **kw)
+    _run("aclnnB200BlockQuantGroupedMatmul", x, x_scale, w, w_scale, rows_per_expert,
+         bool(transposed), out, **kw)
     return out
 
 
@@ -378,9 +448,8 @@ def moe_token_permute(tokens, expert_ids, num_experts, scales=None, out=None, sc
         scales_out = torch.empty((out.shape[0], scales.shape[1]), dtype=torch.float32, device=dev)
     place = torch.empty((T, k), dtype=torch.int32, device=dev)
     counts = torch.empty((num_experts,), dtype=torch.int64, device=dev)
-    _check(tokens, expert_ids, scales, out, scales_out)
-    call("aclnnB200MoeTokenPermute", AclTensor(tokens), AclTensor(expert_ids), _opt(scales), AclTensor(out), _opt(scales_out), AclTensor(place),
-         AclTensor(counts), **kw)
+    _run("aclnnB200MoeTokenPermute", tokens, expert_ids, scales, out, scales_out, place,
+         counts, **kw)
     return (out, place, counts) if scales is None else (out, place, counts, scales_out)
 
 
@@ -388,8 +457,7 @@ def moe_token_permute_grad(grad_rows, place, **kw):
     """The gradient of moe_token_permute's tokens: the sum of each token's rows of grad_rows."""
     import torch
     out = torch.empty((place.shape[0], grad_rows.shape[1]), dtype=grad_rows.dtype, device=grad_rows.device)
-    _check(grad_rows, place)
-    call("aclnnB200MoeTokenPermuteGrad", AclTensor(grad_rows), AclTensor(place), AclTensor(out), **kw)
+    _run("aclnnB200MoeTokenPermuteGrad", grad_rows, place, out, **kw)
     return out
 
 
@@ -397,8 +465,7 @@ def moe_token_unpermute(rows, place, probs=None, **kw):
     """rows [R,H], place int32 [T,k], probs [T,k] -> out [T,H]: the weighted sum of each token's rows."""
     import torch
     out = torch.empty((place.shape[0], rows.shape[1]), dtype=rows.dtype, device=rows.device)
-    _check(rows, place, probs)
-    call("aclnnB200MoeTokenUnpermute", AclTensor(rows), AclTensor(place), _opt(probs), AclTensor(out), **kw)
+    _run("aclnnB200MoeTokenUnpermute", rows, place, probs, out, **kw)
     return out
 
 
@@ -409,6 +476,5 @@ def moe_token_unpermute_grad(grad_out, rows, place, probs, out=None, **kw):
     if out is None:
         out = torch.zeros_like(rows)
     dprobs = torch.empty_like(probs)
-    _check(grad_out, rows, place, probs, out)
-    call("aclnnB200MoeTokenUnpermuteGrad", AclTensor(grad_out), AclTensor(rows), AclTensor(place), AclTensor(probs), AclTensor(out), AclTensor(dprobs), **kw)
+    _run("aclnnB200MoeTokenUnpermuteGrad", grad_out, rows, place, probs, out, dprobs, **kw)
     return out, dprobs

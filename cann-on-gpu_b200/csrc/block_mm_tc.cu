@@ -20,6 +20,9 @@
 // re-laid.  Experts: each CTA scans the row counts on the device into a table of row and tile starts, so the host never sees
 // them; no tile crosses an expert.  Warps: 0 = TMA producer, 1 = MMA issuer and tensor-memory owner, the others = epilogue.
 // Every wait is bounded and records a code in the device status word.
+#include <algorithm>
+
+#include "launch_utils.h"
 #include "tc_common.cuh"
 
 namespace qmm {
@@ -428,12 +431,6 @@ bool make_map3(CUtensorMap *tm, const void *ptr, uint64_t cols, uint64_t rows, u
               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-int bm_sm_count() {
-    int dev = 0, sms = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0) return 148;
-    return sms;
-}
-
 template <bool ROWS_ON_LANES, int NT> cudaError_t launch_form(const BlockMmArgs &a, int split, cudaStream_t s) {
     using S = BmShape<ROWS_ON_LANES, NT>;
     const int E = a.experts > 0 ? (int)a.experts : 1;
@@ -451,19 +448,10 @@ template <bool ROWS_ON_LANES, int NT> cudaError_t launch_form(const BlockMmArgs 
     // tiles: each expert with rows adds at most one partly filled row tile
     const int64_t full = (a.M + S::ROW_TILE - 1) / S::ROW_TILE, most = a.experts > 0 ? std::min<int64_t>(a.M, full + E - 1) : full;
     const int64_t tiles = most * p.n_tiles;
-    const int64_t grid = split > 1 ? tiles * split : std::min<int64_t>(tiles, bm_sm_count());
-    auto kernel = block_mm_tc_kernel<ROWS_ON_LANES, NT>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::TOTAL);
+    const int64_t grid = split > 1 ? tiles * split : std::min<int64_t>(tiles, sm_count());
+    cudaError_t e = allow_smem<block_mm_tc_kernel<ROWS_ON_LANES, NT>>(S::TOTAL);
     if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)grid); cfg.blockDim = dim3(BM_THREADS); cfg.dynamicSmemBytes = S::TOTAL; cfg.stream = s;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = (unsigned)split; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr; cfg.numAttrs = split > 1 ? 2 : 1;
-    e = cudaLaunchKernelEx(&cfg, kernel, tx, tw, p, idesc);
+    e = launch_chained(block_mm_tc_kernel<ROWS_ON_LANES, NT>, (unsigned)grid, BM_THREADS, S::TOTAL, (unsigned)split, s, tx, tw, p, idesc);
     if (e == cudaSuccess) count_launch();
     return e;
 }
@@ -484,7 +472,7 @@ cudaError_t launch_block_mm_tc(const BlockMmArgs &a, cudaStream_t s) {
     const int64_t nkb = (a.K + BM_BK - 1) / BM_BK, cols = (a.N + 127) / 128, full = (a.M + nt - 1) / nt;
     const int64_t tiles = (a.experts > 0 ? std::min<int64_t>(a.M, full + a.experts - 1) : full) * cols;
     int split = 1;
-    while (split < 8 && tiles * split * 2 <= bm_sm_count() && split * 4 <= nkb) split *= 2;
+    while (split < 8 && tiles * split * 2 <= sm_count() && split * 4 <= nkb) split *= 2;
     switch (nt) {
         case 16: return launch_form<false, 16>(a, split, s);
         case 32: return launch_form<false, 32>(a, split, s);

@@ -1,0 +1,54 @@
+// Host-side launch helpers: per-device facts that are looked up once per process.
+#pragma once
+
+#include <atomic>
+
+#include <cuda_runtime.h>
+
+namespace qmm {
+
+inline int current_device() {
+    int dev = 0;
+    return cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64 ? dev : 0;
+}
+inline int sm_count() {
+    static std::atomic<int> sms[64];
+    const int dev = current_device();
+    int n = sms[dev].load(std::memory_order_relaxed);
+    if (n == 0) {
+        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
+        sms[dev].store(n, std::memory_order_relaxed);
+    }
+    return n;
+}
+// Lets `Kernel` use `bytes` of dynamic shared memory (one value per kernel) on the current device.
+template <auto Kernel> cudaError_t allow_smem(int bytes) {
+    static std::atomic<bool> done[64];
+    const int dev = current_device();
+    if (done[dev].load(std::memory_order_acquire)) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done[dev].store(true, std::memory_order_release);
+    return e;
+}
+// Launch that may start while the kernel before it on the stream drains (the kernel waits with griddepcontrol.wait
+// before it touches global memory), as clusters of `cluster` CTAs.
+template <typename... P, typename... A>
+cudaError_t launch_chained(void (*kernel)(P...), unsigned grid, unsigned threads, size_t smem, unsigned cluster, cudaStream_t s, A... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+
+}  // namespace qmm

@@ -4,6 +4,7 @@
 // place -1 and no row.  Everything is a stable counting sort and row copies: no atomics whose order could show, sums in
 // fp32 in the order of j.
 #include "device_utils.cuh"
+#include "launch_utils.h"
 
 namespace qmm {
 namespace {
@@ -111,12 +112,12 @@ __global__ void __launch_bounds__(256) moe_scatter_kernel(const U *tokens, const
     const int lane = threadIdx.x & 31;
     const int64_t t = w / segs, seg = w - t * segs;
     if (t >= T) return;
-    const int32_t p0 = lane < k ? __ldg(place + t * k + lane) : -1, p1 = lane + 32 < k ? __ldg(place + t * k + lane + 32) : -1;
     U v[4];
     const int64_t u0 = seg * 128 + lane;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
         if (u0 + 32 * i < units) v[i] = __ldg(tokens + t * units + u0 + 32 * i);
+    const int32_t p0 = lane < k ? __ldg(place + t * k + lane) : -1, p1 = lane + 32 < k ? __ldg(place + t * k + lane + 32) : -1;
     for (int j = 0; j < k; ++j) {
         const int64_t r = __shfl_sync(0xffffffffu, j < 32 ? p0 : p1, j & 31);
         if (r < 0) continue;
@@ -135,6 +136,58 @@ __global__ void __launch_bounds__(256) moe_scatter_kernel(const U *tokens, const
     }
 }
 
+// ---- few pairs: one launch -----------------------------------------------------------------------
+// A CTA per token finds the places of its pairs itself, by counting among all pairs those of a smaller expert and the
+// earlier ones of the same; the first CTA also counts the rows per expert.  Up to SMALL_PAIRS pairs that takes less than a
+// second launch.
+constexpr int SMALL_PAIRS = 2048;
+template <typename U>
+__global__ void __launch_bounds__(256) moe_small_permute_kernel(const void *ids, bool ids64, int E, const U *tokens, const float *scales, int32_t *place,
+                                                                int64_t *counts, U *rows, float *scales_out, int T, int k, int64_t units, int64_t S) {
+    __shared__ int ex[SMALL_PAIRS];
+    __shared__ int hist[MOE_MAX_EXPERTS];
+    __shared__ int at[MOE_MAX_TOPK];
+    const int N = T * k, t = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    U first{};
+    if (t < T && tid < units) first = __ldg(tokens + (int64_t)t * units + tid);
+    for (int i = tid; i < N; i += 256) {
+        const int e = expert_of(ids, ids64, i, E);
+        ex[i] = e < 0 ? E : e;
+    }
+    if (t == 0)
+        for (int i = tid; i < E; i += 256) hist[i] = 0;
+    __syncthreads();
+    if (t == 0) {
+        for (int i = tid; i < N; i += 256)
+            if (ex[i] < E) atomicAdd(&hist[ex[i]], 1);    // integers: the order does not show
+        __syncthreads();
+        for (int i = tid; i < E; i += 256) counts[i] = hist[i];
+    }
+    if (t >= T) return;                                   // a launch without tokens only clears the counts
+    for (int j = warp; j < k; j += 8) {
+        const int self = t * k + j, e = ex[self];
+        int n = 0;
+        for (int i = lane; i < N; i += 32) n += ex[i] < e || (ex[i] == e && i < self);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+        if (lane == 0) {
+            at[j] = e < E ? n : -1;
+            place[self] = at[j];
+        }
+    }
+    __syncthreads();
+    for (int64_t u = tid; u < units; u += 256) {
+        const U v = u == tid ? first : __ldg(tokens + (int64_t)t * units + u);
+        for (int j = 0; j < k; ++j)
+            if (at[j] >= 0) rows[at[j] * units + u] = v;
+    }
+    for (int64_t c = tid; c < S; c += 256) {
+        const float sc = __ldg(scales + (int64_t)t * S + c);
+        for (int j = 0; j < k; ++j)
+            if (at[j] >= 0) scales_out[at[j] * S + c] = sc;
+    }
+}
+
 // ---- 16 bytes of a row as floats -----------------------------------------------------------------
 // EPV elements per lane: consecutive with VEC (one 16-byte access), else 32 apart (lane-contiguous scalar accesses).
 template <int T> constexpr int epv() { return T == ET_F32 ? 4 : 8; }
@@ -150,17 +203,23 @@ template <int T, bool VEC> struct RowPiece {
                 for (int i = 0; i < N; ++i) f[i] = 0.f;
                 return;
             }
-            const uint4 v = __ldg(reinterpret_cast<const uint4 *>((const char *)p + (row * H + col(seg, lane, 0)) * (T == ET_F32 ? 4 : 2)));
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if constexpr (T == ET_F32) f[i] = __uint_as_float(w[i]);
-                else if constexpr (T == ET_BF16) { f[2 * i] = __uint_as_float(w[i] << 16); f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u); }
-                else { f[2 * i] = __half2float(__ushort_as_half((unsigned short)(w[i] & 0xFFFFu))); f[2 * i + 1] = __half2float(__ushort_as_half((unsigned short)(w[i] >> 16))); }
-            }
+            widen(fetch(p, row, H, seg, lane), f);
         } else {
 #pragma unroll
             for (int i = 0; i < N; ++i) f[i] = col(seg, lane, i) < H ? load_as_float(p, T, row * H + col(seg, lane, i)) : 0.f;
+        }
+    }
+    // The same in two steps, so that several rows' loads are in flight before the first is used (VEC only).
+    static __device__ __forceinline__ uint4 fetch(const void *p, int64_t row, int64_t H, int64_t seg, int lane) {
+        return __ldg(reinterpret_cast<const uint4 *>((const char *)p + (row * H + col(seg, lane, 0)) * (T == ET_F32 ? 4 : 2)));
+    }
+    static __device__ __forceinline__ void widen(const uint4 &v, float (&f)[N]) {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (T == ET_F32) f[i] = __uint_as_float(w[i]);
+            else if constexpr (T == ET_BF16) { f[2 * i] = __uint_as_float(w[i] << 16); f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u); }
+            else { f[2 * i] = __half2float(__ushort_as_half((unsigned short)(w[i] & 0xFFFFu))); f[2 * i + 1] = __half2float(__ushort_as_half((unsigned short)(w[i] >> 16))); }
         }
     }
     static __device__ __forceinline__ void store(void *p, int64_t row, int64_t H, int64_t seg, int lane, const float (&f)[N]) {
@@ -183,7 +242,8 @@ template <int T, bool VEC> struct RowPiece {
 };
 
 // ---- weighted sum of a token's rows --------------------------------------------------------------
-// A warp takes 32 x 16 bytes of one token's output and sums them over the token's rows.
+// A warp takes 32 x 16 bytes of one token's output and sums them over the token's rows, GATHER_J rows in flight.
+constexpr int GATHER_J = 8;
 template <int T, bool VEC>
 __global__ void __launch_bounds__(256) moe_gather_kernel(const void *rows, const int32_t *place, const void *probs, int probs_type, void *out,
                                                          int64_t n_tokens, int k, int64_t R, int64_t H, int64_t segs) {
@@ -193,19 +253,43 @@ __global__ void __launch_bounds__(256) moe_gather_kernel(const void *rows, const
     const int64_t t = w / segs, seg = w - t * segs;
     if (t >= n_tokens) return;
     float acc[P::N] = {};
+    const bool mine = P::col(seg, lane, 0) < H;
     for (int j0 = 0; j0 < k; j0 += 32) {
         const bool has = j0 + lane < k;
-        const int32_t pl = has ? __ldg(place + t * k + j0 + lane) : -1;
+        int32_t pl = has ? __ldg(place + t * k + j0 + lane) : -1;
+        if (pl >= R) pl = -1;
         const float pr = has && probs ? load_as_float(probs, probs_type, t * k + j0 + lane) : 1.f;
         const int n = k - j0 < 32 ? k - j0 : 32;
-        for (int j = 0; j < n; ++j) {
-            const int32_t r = __shfl_sync(0xffffffffu, pl, j);
-            const float f = __shfl_sync(0xffffffffu, pr, j);
-            if (r < 0 || r >= R) continue;
-            float v[P::N];
-            P::load(rows, r, H, seg, lane, v);
+        for (int j1 = 0; j1 < n; j1 += GATHER_J) {
+            if constexpr (VEC) {
+                uint4 v[GATHER_J];
 #pragma unroll
-            for (int i = 0; i < P::N; ++i) acc[i] += f * v[i];
+                for (int j = 0; j < GATHER_J; ++j) {
+                    const int32_t r = __shfl_sync(0xffffffffu, pl, (j1 + j) & 31);
+                    if (j1 + j < n && r >= 0 && mine) v[j] = P::fetch(rows, r, H, seg, lane);
+                }
+#pragma unroll
+                for (int j = 0; j < GATHER_J; ++j) {
+                    const int32_t r = __shfl_sync(0xffffffffu, pl, (j1 + j) & 31);
+                    const float f = __shfl_sync(0xffffffffu, pr, (j1 + j) & 31);
+                    if (j1 + j < n && r >= 0 && mine) {
+                        float x[P::N];
+                        P::widen(v[j], x);
+#pragma unroll
+                        for (int i = 0; i < P::N; ++i) acc[i] += f * x[i];
+                    }
+                }
+            } else {
+                for (int j = j1; j < n && j < j1 + GATHER_J; ++j) {
+                    const int32_t r = __shfl_sync(0xffffffffu, pl, j);
+                    const float f = __shfl_sync(0xffffffffu, pr, j);
+                    if (r < 0) continue;
+                    float x[P::N];
+                    P::load(rows, r, H, seg, lane, x);
+#pragma unroll
+                    for (int i = 0; i < P::N; ++i) acc[i] += f * x[i];
+                }
+            }
         }
     }
     P::store(out, t, H, seg, lane, acc);
@@ -235,12 +319,25 @@ __global__ void __launch_bounds__(256) moe_gather_grad_kernel(const void *dout, 
         }
         for (int64_t seg = warp; seg < segs; seg += warps) {
             float g[P::N];
+            uint4 raw[GRAD_J];
+            if constexpr (VEC) {
+                if (P::col(seg, lane, 0) < H) {
+#pragma unroll
+                    for (int j = 0; j < GRAD_J; ++j)
+                        if (pl[j] >= 0) raw[j] = P::fetch(rows, pl[j], H, seg, lane);
+                }
+            }
             P::load(dout, t, H, seg, lane, g);
 #pragma unroll
             for (int j = 0; j < GRAD_J; ++j) {
                 if (pl[j] < 0) continue;
                 float v[P::N], o[P::N];
-                P::load(rows, pl[j], H, seg, lane, v);
+                if constexpr (VEC) {
+                    if (P::col(seg, lane, 0) >= H) continue;
+                    P::widen(raw[j], v);
+                } else {
+                    P::load(rows, pl[j], H, seg, lane, v);
+                }
 #pragma unroll
                 for (int i = 0; i < P::N; ++i) { dot[j] += g[i] * v[i]; o[i] = pr[j] * g[i]; }
                 P::store(drows, pl[j], H, seg, lane, o);
@@ -264,11 +361,23 @@ __global__ void __launch_bounds__(256) moe_gather_grad_kernel(const void *dout, 
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-template <typename U> cudaError_t launch_scatter(const PermuteArgs &p, cudaStream_t s) {
-    const int64_t units = p.row_bytes / (int64_t)sizeof(U), segs = units > 128 ? (units + 127) / 128 : 1, warps = p.T * segs;
-    if ((warps + 7) / 8 > 0x7fffffffLL) return cudaErrorInvalidValue;
-    moe_scatter_kernel<U><<<(unsigned)((warps + 7) / 8), 256, 0, s>>>((const U *)p.tokens, p.scales, p.place, (U *)p.rows, p.scales_out, p.T, (int)p.k,
-                                                                     units, p.S, segs);
+template <typename U> cudaError_t launch_permute(const PermuteArgs &p, cudaStream_t s) {
+    const int64_t units = p.row_bytes / (int64_t)sizeof(U), N = p.T * p.k;
+    if (N <= SMALL_PAIRS) {
+        moe_small_permute_kernel<U><<<(unsigned)(p.T > 0 ? p.T : 1), 256, 0, s>>>(p.ids, p.ids64, (int)p.E, (const U *)p.tokens, p.scales, p.place, p.counts,
+                                                                                 (U *)p.rows, p.scales_out, (int)p.T, (int)p.k, units, p.S);
+        count_launch();
+        return cudaGetLastError();
+    }
+    cudaError_t e = allow_smem<moe_sort_kernel>((SORT_WARPS + 1) * MOE_MAX_EXPERTS * 4);
+    if (e != cudaSuccess) return e;
+    moe_sort_kernel<<<SORT_CTAS, SORT_WARPS * 32, (size_t)(SORT_WARPS + 1) * p.E * 4, s>>>(p.ids, p.ids64, p.place, p.counts, N, (int)p.E);
+    count_launch();
+    e = cudaGetLastError();
+    if (e != cudaSuccess || (units == 0 && p.S == 0)) return e;
+    const int64_t segs = units > 128 ? (units + 127) / 128 : 1, ctas = (p.T * segs + 7) / 8;
+    if (ctas > 0x7fffffffLL) return cudaErrorInvalidValue;
+    moe_scatter_kernel<U><<<(unsigned)ctas, 256, 0, s>>>((const U *)p.tokens, p.scales, p.place, (U *)p.rows, p.scales_out, p.T, (int)p.k, units, p.S, segs);
     count_launch();
     return cudaGetLastError();
 }
@@ -276,18 +385,11 @@ template <typename U> cudaError_t launch_scatter(const PermuteArgs &p, cudaStrea
 }  // namespace
 
 cudaError_t launch_moe_permute(const PermuteArgs &p, cudaStream_t s) {
-    const size_t smem = (size_t)(SORT_WARPS + 1) * p.E * 4;
-    cudaError_t e = cudaFuncSetAttribute(moe_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (SORT_WARPS + 1) * MOE_MAX_EXPERTS * 4);
-    if (e != cudaSuccess) return e;
-    moe_sort_kernel<<<SORT_CTAS, SORT_WARPS * 32, smem, s>>>(p.ids, p.ids64, p.place, p.counts, p.T * p.k, (int)p.E);
-    count_launch();
-    e = cudaGetLastError();
-    if (e != cudaSuccess || p.T == 0 || (p.row_bytes == 0 && p.S == 0)) return e;
     const uintptr_t all = reinterpret_cast<uintptr_t>(p.tokens) | reinterpret_cast<uintptr_t>(p.rows) | (uintptr_t)p.row_bytes;
-    if (all % 16 == 0) return launch_scatter<uint4>(p, s);
-    if (all % 4 == 0) return launch_scatter<uint32_t>(p, s);
-    if (all % 2 == 0) return launch_scatter<uint16_t>(p, s);
-    return launch_scatter<uint8_t>(p, s);
+    if (all % 16 == 0) return launch_permute<uint4>(p, s);
+    if (all % 4 == 0) return launch_permute<uint32_t>(p, s);
+    if (all % 2 == 0) return launch_permute<uint16_t>(p, s);
+    return launch_permute<uint8_t>(p, s);
 }
 
 cudaError_t launch_moe_unpermute(const void *rows, int type, const int32_t *place, const void *probs, int probs_type, void *out,

@@ -1,0 +1,183 @@
+// Pieces shared by the two tensor-core forms of the block-scaled fp8 matmul (block_mm_tc.cu, block_mm_pair.cu).
+#pragma once
+
+#include "launch_utils.h"
+#include "tc_common.cuh"
+
+namespace qmm {
+namespace {
+
+constexpr int BM_LANES = 128, BM_BK = 128, BM_EPI_WARPS = 8, BM_THREADS = 64 + BM_EPI_WARPS * 32;
+constexpr int BM_TABLE_BYTES = (2 * BLOCK_MM_MAX_EXPERTS + 4) * 4;   // row starts [E + 1], tile ends [E]
+
+struct BmParams {
+    const float *xs, *ws;
+    const int64_t *counts;      // [E] on the device, or null
+    void *out;
+    int out_type, vec_out;
+    int M, N, nkb, nb, E;       // E >= 1 (dense: 1)
+    int n_tiles, w_nk, split;
+};
+
+// D fp32, A / B formats (0 = e4m3, 1 = e5m2), A and B MN-major flags.
+constexpr uint32_t bm_idesc(int a_fmt, int b_fmt, int a_mn, int b_mn, int m, int n) {
+    return (1u << 4) | ((uint32_t)a_fmt << 7) | ((uint32_t)b_fmt << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
+           ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *tm, uint32_t bar, int x, int y, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+        ::"r"(dst), "l"(tm), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
+}
+// tcgen05.ld of 8 or 16 columns without the wait; the wait takes the registers so that no use moves in front of it.
+template <int N> __device__ __forceinline__ void bm_ld(uint32_t taddr, uint32_t (&r)[N]) {
+    if constexpr (N == 16)
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+                       "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(taddr) : "memory");
+    else
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(taddr) : "memory");
+}
+template <int N> __device__ __forceinline__ void bm_ld_wait(uint32_t (&r)[N]) {
+    if constexpr (N == 16)
+        asm volatile("tcgen05.wait::ld.sync.aligned;"
+                     : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
+                       "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]) :: "memory");
+    else
+        asm volatile("tcgen05.wait::ld.sync.aligned;"
+                     : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]) :: "memory");
+}
+__device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(lo), "r"(hi));
+    return v;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float &lo, float &hi) {
+    uint32_t a, b;
+    asm("mov.b64 {%0, %1}, %2;" : "=r"(a), "=r"(b) : "l"(v));
+    lo = __uint_as_float(a);
+    hi = __uint_as_float(b);
+}
+// Two fp32 fused multiply-adds in one instruction.
+__device__ __forceinline__ void fma2(uint64_t &acc, uint64_t a, uint64_t b) { asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(a), "l"(b)); }
+
+// One lane of a converged warp; the compiler keeps the operands of what it guards in uniform registers (a branch on the
+// lane number does not: a K block's four products then took about 800 cycles to issue).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) :: "memory");
+    return ok != 0;
+}
+// Bounded wait of a whole warp, with one answer for all lanes.  CLUSTER also acquires what another CTA released.
+template <bool CLUSTER = false>
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, unsigned code) {
+    unsigned long long t0 = 0;
+    for (unsigned it = 0;; ++it) {
+        uint32_t ok;
+        if constexpr (CLUSTER)
+            asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                         : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+        else
+            asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                         : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+        if (__all_sync(0xffffffffu, ok != 0)) return true;
+        if ((it & 63u) == 63u) {
+            const unsigned long long t = global_ns();
+            if (t0 == 0) t0 = t;
+            const bool late = t - t0 > WAIT_LIMIT_NS;
+            if (late) {
+                *abort_flag = 1;
+                atomicCAS(&g_tc_status, 0u, code);
+            }
+            if (__any_sync(0xffffffffu, late || *abort_flag)) return false;
+        }
+    }
+}
+// A product or copy in flight is awaited with a limit before the memory it uses goes away.
+__device__ __forceinline__ void bm_drain(uint32_t bar, uint32_t parity) {
+    const unsigned long long t0 = global_ns();
+    while (!mbar_try_wait(bar, parity) && global_ns() - t0 < 50000000ull) {}
+}
+
+__device__ __forceinline__ void bm_cluster_sync() {
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// ---- scales ahead of their blocks ----------------------------------------------------------------
+// One warp copies the scales of each block to a ring in shared memory, SC_AHEAD blocks before they are used: a row's
+// scales are nkb floats apart from the next row's, so a block's 128 are as many cache lines, and when the epilogue warps fetched
+// them (even two blocks ahead) they waited 1000 cycles per block.  The warp reports a block by arriving on the accumulator's own
+// "full" barrier, next to the products' commit, so the epilogue waits once for both.
+constexpr int SC_SLOTS = 16, SC_AHEAD = 8;
+__device__ __forceinline__ void cp_async4(uint32_t dst, const float *src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// The table of a launch, filled by one warp: rows of expert e are row_start[e] .. row_start[e + 1], its tiles end at
+// tile_end[e].  Without counts there is one expert with all M rows.
+template <int ROW_TILE>
+__device__ __forceinline__ void fill_table(const int64_t *counts, int M, int E, int n_tiles, int *row_start, int *tile_end) {
+    const int lane = threadIdx.x & 31;
+            if (!counts) {
+                if (lane == 0) { row_start[0] = 0; row_start[1] = M; tile_end[0] = (M + ROW_TILE - 1) / ROW_TILE * n_tiles; }
+            } else {
+                // counts below 0 count as 0, and rows end at M
+                int rows = 0, tiles = 0;
+                for (int e0 = 0; e0 < E; e0 += 32) {
+                    const int e = e0 + lane;
+                    long long c = e < E ? __ldg((const long long *)counts + e) : 0;
+                    c = c < 0 ? 0 : (c > M ? M : c);
+                    long long end = c;
+    #pragma unroll
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const long long v = __shfl_up_sync(0xffffffffu, end, o);
+                        if (lane >= o) end += v;
+                    }
+                    const long long lo64 = rows + end - c, hi64 = rows + end;
+                    const int lo = (int)(lo64 < M ? lo64 : M), hi = (int)(hi64 < M ? hi64 : M);
+                    int t = (hi - lo + ROW_TILE - 1) / ROW_TILE * n_tiles;
+    #pragma unroll
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const int v = __shfl_up_sync(0xffffffffu, t, o);
+                        if (lane >= o) t += v;
+                    }
+                    if (e < E) { row_start[e] = lo; tile_end[e] = tiles + t; if (e == E - 1) row_start[E] = hi; }
+                    rows = __shfl_sync(0xffffffffu, hi, 31);
+                    tiles += __shfl_sync(0xffffffffu, t, 31);
+                }
+            }
+}
+
+// Tile t in ascending t: expert, first row and rows, first column.
+template <int ROW_TILE, int COL_TILE>
+struct TileWalk {
+    const int *row_start, *tile_end;
+    int e = 0;
+    __device__ __forceinline__ void seek(int tile, int &expert, int &m0, int &rows, int &n0) {
+        while (tile >= tile_end[e]) ++e;
+        const int local = tile - (e ? tile_end[e - 1] : 0), r0 = row_start[e], r1 = row_start[e + 1];
+        const int mt = (r1 - r0 + ROW_TILE - 1) / ROW_TILE;
+        const int nt = local / mt;
+        m0 = r0 + (local - nt * mt) * ROW_TILE;
+        rows = r1 - m0 < ROW_TILE ? r1 - m0 : ROW_TILE;
+        n0 = nt * COL_TILE;
+        expert = e;
+    }
+};
+
+// 3-D map of E matrices of `rows` rows of `cols` bytes.
+bool make_map3(CUtensorMap *tm, const void *ptr, uint64_t cols, uint64_t rows, uint64_t E, uint32_t box_cols, uint32_t box_rows) {
+    EncodeFn fn = encode_fn();
+    if (!fn) return false;
+    cuuint64_t dims[3] = {cols, rows, E}, strides[2] = {cols, cols * rows};
+    cuuint32_t box[3] = {box_cols, box_rows, 1}, estr[3] = {1, 1, 1};
+    return fn(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void *>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+}  // namespace
+}  // namespace qmm

@@ -1,0 +1,343 @@
+// Block-scaled fp8 matmul for many rows: a pair of CTAs (cta_group::2) per tile of 256 rows x 256 columns.
+//
+// Each CTA of the pair loads 128 rows of x and 128 of the tile's weight columns per block of 128 k's; one tcgen05.mma of M = 256,
+// N = 256 reads both CTAs' shared memory and leaves 128 x 256 sums in each CTA's tensor memory.  A weight byte
+// fetched once thus serves 256 rows and a byte of x 256 columns: 32 KB per CTA and block where a single CTA's 128 x 256 tile needs 48 KB.
+//
+// The block's sums leave tensor memory before the next block's are added (the scales are arbitrary fp32 numbers): two
+// accumulators of 256 columns alternate, and sixteen epilogue warps per CTA fold each into 64 fp32 registers a
+// thread, acc += part * (xs[row] * ws[128-column block]), two multiply-adds per instruction.  What bounds the kernel is the
+// round trip of an accumulator -- products, commit, fold, hand-back across the pair, next products -- hence many epilogue warps
+// with a short fold each, scales that are there before the block, and a hand-back before the last multiply-adds.
+//
+// Roles per CTA: warp 0 = TMA producer of its own halves; warp 1 = in the leader the MMA issuer, in the other CTA the relay
+// that tells the leader its stage is filled; warp 2 = scales; warps 4-19 = epilogue.  Waits are bounded, and the pair meets at a cluster
+// barrier before either CTA's memory goes away.
+#include "block_mm_common.cuh"
+
+namespace qmm {
+namespace {
+
+constexpr int BP_STAGES = 5, BP_NBUF = 2, BP_ROWS = 256, BP_COLS = 256, BP_EPI = 16, BP_THREADS = 128 + BP_EPI * 32;
+struct BpSmem {
+    static constexpr int X_BYTES = 128 * BM_BK, W_BYTES = 128 * BM_BK, STAGE = X_BYTES + W_BYTES;
+    static constexpr int TABLE_OFF = BP_STAGES * STAGE;
+    static constexpr int OUT_OFF = TABLE_OFF + BM_TABLE_BYTES;      // 32 rows x 64 bytes per epilogue warp
+    static constexpr int SC_OFF = OUT_OFF + BP_EPI * 2048;          // per slot: 128 row scales, 2 of the weight's blocks
+    static constexpr int SC_SLOT = 130 * 4;
+    static constexpr int BAR_OFF = (SC_OFF + SC_SLOTS * SC_SLOT + 7) / 8 * 8;
+    static constexpr int NUM_BARS = 2 * BP_STAGES + 2 * BP_NBUF;
+    static constexpr int MISC_OFF = BAR_OFF + NUM_BARS * 8;
+    static constexpr int TOTAL = MISC_OFF + 16 + 1024;
+};
+static_assert(BpSmem::TOTAL <= 232448, "shared memory budget of one CTA");
+
+__device__ __forceinline__ void bp_mma(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+}
+// Arrives on the barrier at this offset in both CTAs when the products issued so far are done.
+__device__ __forceinline__ void bp_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                 ::"r"(bar), "h"((uint16_t)3) : "memory");
+}
+__device__ __forceinline__ uint32_t bp_at(uint32_t addr, uint32_t cta) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(cta));
+    return a;
+}
+// (Without a release at cluster scope: what it reports -- tensor memory read, a copy landed -- is not the thread's own
+// memory traffic, and waiting for that to drain took about 1500 cycles per block.)
+__device__ __forceinline__ void bp_arrive(uint32_t cluster_bar) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+
+__global__ void __launch_bounds__(BP_THREADS, 1)
+block_mm_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w, const BmParams p, const uint32_t idesc) {
+    using S = BpSmem;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t *gen_base = smem_raw + (base - smem_u32(smem_raw));
+    auto x_tile = [&](int s) { return base + s * S::STAGE; };
+    auto w_tile = [&](int s) { return base + s * S::STAGE + S::X_BYTES; };
+    auto bar_full = [&](int s) { return base + S::BAR_OFF + 8 * s; };        // in the leader: of both CTAs' stages
+    auto bar_empty = [&](int s) { return base + S::BAR_OFF + 8 * (BP_STAGES + s); };
+    auto bar_acc_full = [&](int a) { return base + S::BAR_OFF + 8 * (2 * BP_STAGES + a); };              // products and scales
+    auto bar_acc_empty = [&](int a) { return base + S::BAR_OFF + 8 * (2 * BP_STAGES + BP_NBUF + a); };   // leader: both CTAs' epilogues
+    int *row_start = reinterpret_cast<int *>(gen_base + S::TABLE_OFF), *tile_end = row_start + p.E + 1;
+    volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(gen_base + S::MISC_OFF);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(gen_base + S::MISC_OFF + 4);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = (int)blockIdx.x & 1;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < BP_STAGES; ++s) { mbar_init(bar_full(s), rank == 0 ? 2 : 1); mbar_init(bar_empty(s), 1); }
+        for (int a = 0; a < BP_NBUF; ++a) { mbar_init(bar_acc_full(a), 2); mbar_init(bar_acc_empty(a), 2 * BP_EPI); }
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        fence_proxy_async();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void *)tmem_slot)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // everything below reads or writes global memory
+    if (warp == 0) fill_table<BP_ROWS>(p.counts, p.M, p.E, p.n_tiles, row_start, tile_end);
+    tc_fence_before();
+    bm_cluster_sync();                                    // both CTAs' barriers and tensor memory are there
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    const int tiles = tile_end[p.E - 1];
+    const int first = (int)blockIdx.x >> 1, step = (int)gridDim.x >> 1;
+    TileWalk<BP_ROWS, BP_COLS> walk{row_start, tile_end};
+    int issued = 0;                                       // warp 0: stages filled; the leader's warp 1: blocks multiplied
+
+    if (warp == 0) {
+        int s = 0;
+        uint32_t ph = 1;                                  // of bar_empty: the first round finds the stages free
+        bool ok = true;
+        for (int tile = first; tile < tiles && ok; tile += step) {
+            int e, m0, rows, n0;
+            walk.seek(tile, e, m0, rows, n0);
+            m0 += rank * 128;
+            n0 += rank * 128;
+            for (int kb = 0; kb < p.nkb; ++kb) {
+                if (!warp_wait(bar_empty(s), ph, abort_flag, 0x611u)) { ok = false; break; }
+                if (elect_one()) {
+                    mbar_expect_tx(bar_full(s), S::STAGE);
+                    const int k = kb * BM_BK;
+                    tma_load_2d(x_tile(s), &tm_x, bar_full(s), k, m0);
+                    tma_load_3d(w_tile(s), &tm_w, bar_full(s), p.w_nk ? k : n0, p.w_nk ? n0 : k, e);
+                }
+                __syncwarp();
+                ++issued;
+                if (++s == BP_STAGES) { s = 0; ph ^= 1u; }
+            }
+        }
+    } else if (warp == 1) {
+        const uint32_t w_step = p.w_nk ? 32u : 4096u, w_lbo = p.w_nk ? 16u : 16384u;
+        const uint64_t x_desc = smem_desc(x_tile(0), 16, 1024), w_desc = smem_desc(w_tile(0), w_lbo, 1024);
+        int s = 0, a = 0;
+        uint32_t ph = 0, aph = 1;
+        bool ok = true;
+        for (int tile = first; tile < tiles && ok; tile += step) {
+            for (int kb = 0; kb < p.nkb; ++kb) {
+                if (rank == 0) {
+                    if (!warp_wait<true>(bar_full(s), ph, abort_flag, 0x613u) || !warp_wait<true>(bar_acc_empty(a), aph, abort_flag, 0x612u)) { ok = false; break; }
+                    tc_fence_after();
+                    const uint32_t d = tmem_base + (uint32_t)(a * BP_COLS);
+                    const uint64_t xd = x_desc + (uint32_t)(s * (S::STAGE >> 4)), wd = w_desc + (uint32_t)(s * (S::STAGE >> 4));
+                    if (elect_one()) {
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk) bp_mma(d, xd + (uint32_t)(kk * 2), wd + kk * (w_step >> 4), idesc, kk > 0 ? 1u : 0u);
+                        bp_commit(bar_acc_full(a));
+                        bp_commit(bar_empty(s));
+                    }
+                    __syncwarp();
+                    ++issued;
+                    a ^= 1;
+                    if (a == 0) aph ^= 1u;
+                } else {
+                    if (!warp_wait(bar_full(s), ph, abort_flag, 0x615u)) { ok = false; break; }
+                    if (elect_one()) bp_arrive(bp_at(bar_full(s), 0));
+                    __syncwarp();
+                }
+                if (++s == BP_STAGES) { s = 0; ph ^= 1u; }
+            }
+        }
+    } else if (warp == 2) {
+        // scales: the copies run SC_AHEAD blocks in front of the reports.  Slots are reused 16 blocks later, and a report
+        // for block i waits for block i - 2 to be complete, by when block i - 4 has been folded.
+        TileWalk<BP_ROWS, BP_COLS> ahead{row_start, tile_end};
+        int atile = first, akb = 0, slot = 0, rows = 0;
+        const float *xsp[4], *wsp[2];
+        const int ws_step = p.w_nk ? 1 : p.nb;
+        bool w_ok = false;
+        auto copy_next = [&] {                            // one commit group per block, empty behind the last tile
+            if (atile < tiles) {
+                if (akb == 0) {
+                    int e, m0, n0;
+                    ahead.seek(atile, e, m0, rows, n0);
+                    rows -= rank * 128;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) xsp[i] = p.xs + (int64_t)(m0 + rank * 128 + lane + 32 * i) * p.nkb;
+                    const int nblk = n0 / 128 + (lane & 1);
+                    w_ok = lane < 2 && nblk < p.nb;
+                    wsp[0] = p.ws + (int64_t)e * p.nkb * p.nb + (p.w_nk ? (int64_t)nblk * p.nkb : nblk);
+                }
+                const uint32_t dst = base + S::SC_OFF + (uint32_t)slot * S::SC_SLOT;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (lane + 32 * i < rows) cp_async4(dst + (lane + 32 * i) * 4, xsp[i] + akb);
+                if (w_ok) cp_async4(dst + (128 + lane) * 4, wsp[0] + (int64_t)akb * ws_step);
+                if (++akb == p.nkb) { akb = 0; atile += step; }
+                slot = (slot + 1) & (SC_SLOTS - 1);
+            }
+            cp_async_commit();
+        };
+        for (int i = 0; i < SC_AHEAD; ++i) copy_next();
+        int a = 0;
+        uint32_t ph = 1;                                  // of the accumulator's previous use
+        bool ok = true;
+        for (int tile = first; tile < tiles && ok; tile += step) {
+            for (int kb = 0; kb < p.nkb; ++kb) {
+                if (!warp_wait(bar_acc_full(a), ph, abort_flag, 0x617u)) { ok = false; break; }
+                copy_next();
+                cp_async_wait<SC_AHEAD>();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar_acc_full(a));
+                a ^= 1;
+                if (a == 0) ph ^= 1u;
+            }
+        }
+        cp_async_wait<0>();
+    } else if (warp >= 4) {
+        const int ew = warp - 4, set = ew >> 2, q = warp & 3;
+        constexpr int COLS = BP_COLS / 4, CH = 16, NCH = COLS / CH;
+        const uint32_t tm_lane = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(set * COLS);
+        const uint32_t give = bp_at(bar_acc_empty(0), 0);  // in the leader, of accumulator 0; 8 bytes on, of 1
+        int a = 0, slot = 0;
+        uint32_t ph = 0;
+        bool ok = true;
+        for (int tile = first; tile < tiles && ok; tile += step) {
+            uint64_t acc[COLS / 2];
+#pragma unroll
+            for (int i = 0; i < COLS / 2; ++i) acc[i] = 0ull;
+            for (int kb = 0; kb < p.nkb; ++kb) {
+                if (!warp_wait(bar_acc_full(a), ph, abort_flag, 0x616u)) { ok = false; break; }
+                tc_fence_after();
+                const uint32_t taddr = tm_lane + (uint32_t)(a * BP_COLS);
+                uint32_t v[CH];
+                bm_ld<CH>(taddr, v);
+                const float *sc = reinterpret_cast<const float *>(gen_base + S::SC_OFF + slot * S::SC_SLOT);
+                const float f = sc[q * 32 + lane] * sc[128 + (set >> 1)];
+                const uint64_t f2 = pack2(__float_as_uint(f), __float_as_uint(f));
+#pragma unroll
+                for (int c = 0; c < NCH; ++c) {
+                    bm_ld_wait<CH>(v);
+                    if (c + 1 == NCH) {                   // all of it is in registers: the accumulator is free
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) bp_arrive(give + 8u * (uint32_t)a);
+                    }
+#pragma unroll
+                    for (int i = 0; i < CH; i += 2) fma2(acc[(c * CH + i) / 2], pack2(v[i], v[i + 1]), f2);
+                    if (c + 1 < NCH) bm_ld<CH>(taddr + (c + 1) * CH, v);
+                }
+                slot = (slot + 1) & (SC_SLOTS - 1);
+                a ^= 1;
+                if (a == 0) ph ^= 1u;
+            }
+            if (!ok) break;
+            int e, m0, rows, n0;
+            walk.seek(tile, e, m0, rows, n0);
+            m0 += rank * 128 + q * 32;                    // this warp's rows
+            rows -= rank * 128 + q * 32;
+            const int nc = n0 + set * COLS;
+            if (p.vec_out) {                              // N a multiple of 8, 16-byte aligned
+                // 64 bytes of each row at a time through shared memory, so that a store covers 8 rows and not 32
+                // (units of 16 bytes, their order in a row turned by the row so that neither side meets in a bank)
+                const bool f32 = p.out_type == ET_F32;
+                const int per = f32 ? 16 : 32, unit = f32 ? 4 : 8;    // columns of a pass, of 16 bytes
+                uint4 *box = reinterpret_cast<uint4 *>(gen_base + S::OUT_OFF) + ew * 128;
+#pragma unroll
+                for (int pass = 0; pass < 4; ++pass) {
+                    if (pass >= 2 && !f32) break;
+                    __syncwarp();
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        uint4 w;
+                        if (f32) {
+                            const uint64_t w0 = acc[pass * 8 + 2 * u], w1 = acc[pass * 8 + 2 * u + 1];
+                            w = make_uint4((uint32_t)w0, (uint32_t)(w0 >> 32), (uint32_t)w1, (uint32_t)(w1 >> 32));
+                        } else {
+                            uint32_t h[4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                float f0, f1;
+                                unpack2(acc[(pass & 1) * 16 + 4 * u + i], f0, f1);
+                                if (p.out_type == ET_BF16) { __nv_bfloat162 b = __floats2bfloat162_rn(f0, f1); h[i] = *reinterpret_cast<uint32_t *>(&b); }
+                                else { __half2 b = __floats2half2_rn(f0, f1); h[i] = *reinterpret_cast<uint32_t *>(&b); }
+                            }
+                            w = make_uint4(h[0], h[1], h[2], h[3]);
+                        }
+                        box[lane * 4 + (u ^ ((lane >> 1) & 3))] = w;
+                    }
+                    __syncwarp();
+                    const int col = nc + pass * per + (lane & 3) * unit;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int r = i * 8 + (lane >> 2);
+                        const uint4 t = box[r * 4 + ((lane & 3) ^ ((r >> 1) & 3))];
+                        if (r < rows && col < p.N)
+                            *reinterpret_cast<uint4 *>((uint8_t *)p.out + ((int64_t)(m0 + r) * p.N + col) * (f32 ? 4 : 2)) = t;
+                    }
+                }
+            } else if (lane < rows) {
+                const int64_t at = (int64_t)(m0 + lane) * p.N + nc;
+#pragma unroll
+                for (int i = 0; i < COLS / 2; ++i) {
+                    float f0, f1;
+                    unpack2(acc[i], f0, f1);
+                    if (nc + 2 * i < p.N) store_from_float(p.out, p.out_type, at + 2 * i, f0);
+                    if (nc + 2 * i + 1 < p.N) store_from_float(p.out, p.out_type, at + 2 * i + 1, f1);
+                }
+            }
+            __syncwarp();
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (*abort_flag) {
+        // a wait gave up: copies and products in flight end before the pair's memory goes (each awaited with a limit)
+        if (warp == 0 && lane == 0)
+            for (int j = issued > BP_STAGES ? issued - BP_STAGES : 0; j < issued; ++j) bm_drain(bar_full(j % BP_STAGES), (j / BP_STAGES) & 1);
+        if (warp == 1 && lane == 0)
+            for (int j = issued > BP_NBUF ? issued - BP_NBUF : 0; j < issued; ++j) bm_drain(bar_acc_full(j % BP_NBUF), (j / BP_NBUF) & 1);
+    }
+    bm_cluster_sync();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
+    }
+}
+
+}  // namespace
+
+cudaError_t launch_block_mm_pair(const BlockMmArgs &a, cudaStream_t s) {
+    const int E = a.experts > 0 ? (int)a.experts : 1;
+    CUtensorMap tx, tw;
+    bool ok = make_map(&tx, a.x, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.K, a.M, a.K, BM_BK, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+    ok = ok && (a.w_nk ? make_map3(&tw, a.w, a.K, a.N, E, BM_BK, 128) : make_map3(&tw, a.w, a.N, a.K, E, 128, BM_BK));
+    if (!ok) return cudaErrorInvalidValue;
+    BmParams p{};
+    p.xs = a.xs; p.ws = a.ws; p.counts = a.experts > 0 ? a.group_rows : nullptr; p.out = a.out; p.out_type = a.out_type;
+    p.vec_out = a.N % 8 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
+    p.M = (int)a.M; p.N = (int)a.N; p.nkb = (int)((a.K + BM_BK - 1) / BM_BK); p.nb = (int)((a.N + 127) / 128); p.E = E;
+    p.n_tiles = (int)((a.N + BP_COLS - 1) / BP_COLS); p.w_nk = a.w_nk; p.split = 1;
+    const uint32_t idesc = bm_idesc(a.x_type == ET_E5M2, a.w_type == ET_E5M2, 0, a.w_nk ? 0 : 1, BP_ROWS, BP_COLS);
+    // tiles: each expert with rows adds at most one partly filled row tile
+    const int64_t full = (a.M + BP_ROWS - 1) / BP_ROWS, most = a.experts > 0 ? (a.M < full + E - 1 ? a.M : full + E - 1) : full;
+    const int64_t tiles = most * p.n_tiles, pairs = sm_count() / 2;
+    cudaError_t e = allow_smem<block_mm_pair_kernel>(BpSmem::TOTAL);
+    if (e != cudaSuccess) return e;
+    e = launch_chained(block_mm_pair_kernel, 2 * (unsigned)(tiles < pairs ? tiles : pairs), BP_THREADS, BpSmem::TOTAL, 2, s, tx, tw, p, idesc);
+    if (e == cudaSuccess) count_launch();
+    return e;
+}
+
+unsigned int block_mm_pair_device_status() {
+    unsigned int v = 0;
+    if (cudaMemcpyFromSymbol(&v, g_tc_status, sizeof(v)) != cudaSuccess) return 0xFFFFFFFFu;
+    return v;
+}
+void block_mm_pair_device_status_reset() {
+    const unsigned int z = 0;
+    cudaMemcpyToSymbol(g_tc_status, &z, sizeof(z));
+}
+
+}  // namespace qmm

@@ -22,22 +22,10 @@
 // Every wait is bounded and records a code in the device status word.
 #include <algorithm>
 
-#include "launch_utils.h"
-#include "tc_common.cuh"
+#include "block_mm_common.cuh"
 
 namespace qmm {
 namespace {
-
-constexpr int BM_LANES = 128, BM_BK = 128, BM_EPI_WARPS = 8, BM_THREADS = 64 + BM_EPI_WARPS * 32;
-
-struct BmParams {
-    const float *xs, *ws;
-    const int64_t *counts;      // [E] on the device, or null
-    void *out;
-    int out_type, vec_out;
-    int M, N, nkb, nb, E;       // E >= 1 (dense: 1)
-    int n_tiles, w_nk, split;
-};
 
 // ROWS_ON_LANES: lanes = rows of x, columns = NT weight columns.  Else lanes = 128 weight columns, columns = NT rows of x.
 template <bool ROWS_ON_LANES, int NT>
@@ -49,7 +37,7 @@ struct BmShape {
     static constexpr int SETS = BM_EPI_WARPS / 4, COLS = NT / SETS;    // columns of a thread
     static constexpr int ROW_TILE = ROWS_ON_LANES ? BM_LANES : NT, COL_TILE = ROWS_ON_LANES ? NT : BM_LANES;
     static constexpr int TABLE_OFF = STAGES * STAGE;                   // row starts [E + 1], tile ends [E]
-    static constexpr int FACT_OFF = TABLE_OFF + (2 * BLOCK_MM_MAX_EXPERTS + 4) * 4;
+    static constexpr int FACT_OFF = TABLE_OFF + BM_TABLE_BYTES;
     static constexpr int BAR_OFF = FACT_OFF + BM_EPI_WARPS * COLS * 4;
     static constexpr int NUM_BARS = 2 * STAGES + 2 * NBUF;
     static constexpr int MISC_OFF = BAR_OFF + NUM_BARS * 8;
@@ -63,83 +51,13 @@ __device__ __forceinline__ void bm_mma(uint32_t d_tmem, uint64_t a_desc, uint64_
         "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
         ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
 }
-// D fp32, A / B formats (0 = e4m3, 1 = e5m2), A and B MN-major flags.
-constexpr uint32_t bm_idesc(int a_fmt, int b_fmt, int a_mn, int b_mn, int m, int n) {
-    return (1u << 4) | ((uint32_t)a_fmt << 7) | ((uint32_t)b_fmt << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
-           ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
-}
-__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *tm, uint32_t bar, int x, int y, int z) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
-        ::"r"(dst), "l"(tm), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
-}
-// tcgen05.ld of 8 or 16 columns without the wait; the wait takes the registers so that no use moves in front of it.
-template <int N> __device__ __forceinline__ void bm_ld(uint32_t taddr, uint32_t (&r)[N]) {
-    if constexpr (N == 16)
-        asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-                       "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(taddr) : "memory");
-    else
-        asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(taddr) : "memory");
-}
-template <int N> __device__ __forceinline__ void bm_ld_wait(uint32_t (&r)[N]) {
-    if constexpr (N == 16)
-        asm volatile("tcgen05.wait::ld.sync.aligned;"
-                     : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
-                       "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]) :: "memory");
-    else
-        asm volatile("tcgen05.wait::ld.sync.aligned;"
-                     : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]) :: "memory");
-}
-__device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
-    uint64_t v;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(lo), "r"(hi));
-    return v;
-}
-__device__ __forceinline__ void unpack2(uint64_t v, float &lo, float &hi) {
-    uint32_t a, b;
-    asm("mov.b64 {%0, %1}, %2;" : "=r"(a), "=r"(b) : "l"(v));
-    lo = __uint_as_float(a);
-    hi = __uint_as_float(b);
-}
-// Two fp32 fused multiply-adds in one instruction.
-__device__ __forceinline__ void fma2(uint64_t &acc, uint64_t a, uint64_t b) { asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(a), "l"(b)); }
-
-__device__ __forceinline__ void bm_drain(uint32_t bar, uint32_t parity) {
-    const unsigned long long t0 = global_ns();
-    while (!mbar_try_wait(bar, parity) && global_ns() - t0 < 50000000ull) {}
-}
-
-__device__ __forceinline__ void bm_cluster_sync() {
-    __syncwarp();
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ float ld_cluster_f32(uint32_t local, uint32_t cta) {
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t local, uint32_t cta) {
     uint32_t a;
-    float v;
+    float4 v;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(local), "r"(cta));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
     return v;
 }
-
-// Tile t in ascending t: expert, first row and rows, first column.
-template <int ROW_TILE, int COL_TILE>
-struct TileWalk {
-    const int *row_start, *tile_end;
-    int e = 0;
-    __device__ __forceinline__ void seek(int tile, int &expert, int &m0, int &rows, int &n0) {
-        while (tile >= tile_end[e]) ++e;
-        const int local = tile - (e ? tile_end[e - 1] : 0), r0 = row_start[e], r1 = row_start[e + 1];
-        const int mt = (r1 - r0 + ROW_TILE - 1) / ROW_TILE;
-        const int nt = local / mt;
-        m0 = r0 + (local - nt * mt) * ROW_TILE;
-        rows = r1 - m0 < ROW_TILE ? r1 - m0 : ROW_TILE;
-        n0 = nt * COL_TILE;
-        expert = e;
-    }
-};
 
 template <bool ROWS_ON_LANES, int NT>
 __global__ void __launch_bounds__(BM_THREADS, 1)
@@ -170,34 +88,7 @@ block_mm_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");   // everything below reads or writes global memory
     if (warp == 0) {
-        if (!p.counts) {
-            if (lane == 0) { row_start[0] = 0; row_start[1] = p.M; tile_end[0] = (p.M + S::ROW_TILE - 1) / S::ROW_TILE * p.n_tiles; }
-        } else {
-            // counts below 0 count as 0, and rows end at M
-            int rows = 0, tiles = 0;
-            for (int e0 = 0; e0 < p.E; e0 += 32) {
-                const int e = e0 + lane;
-                long long c = e < p.E ? __ldg((const long long *)p.counts + e) : 0;
-                c = c < 0 ? 0 : (c > p.M ? p.M : c);
-                long long end = c;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const long long v = __shfl_up_sync(0xffffffffu, end, o);
-                    if (lane >= o) end += v;
-                }
-                const long long lo64 = rows + end - c, hi64 = rows + end;
-                const int lo = (int)(lo64 < p.M ? lo64 : p.M), hi = (int)(hi64 < p.M ? hi64 : p.M);
-                int t = (hi - lo + S::ROW_TILE - 1) / S::ROW_TILE * p.n_tiles;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const int v = __shfl_up_sync(0xffffffffu, t, o);
-                    if (lane >= o) t += v;
-                }
-                if (e < p.E) { row_start[e] = lo; tile_end[e] = tiles + t; if (e == p.E - 1) row_start[p.E] = hi; }
-                rows = __shfl_sync(0xffffffffu, hi, 31);
-                tiles += __shfl_sync(0xffffffffu, t, 31);
-            }
-        }
+        fill_table<S::ROW_TILE>(p.counts, p.M, p.E, p.n_tiles, row_start, tile_end);
     }
     tc_fence_before();
     __syncthreads();
@@ -211,15 +102,15 @@ block_mm_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
 
     int issued = 0;                                        // warp 0: stages filled; warp 1: blocks multiplied
     if (warp == 0) {
-        if (lane == 0) {
-            int &it = issued;
-            bool ok = true;
-            for (int tile = first; tile < tiles && ok; tile += step) {
-                int e, m0, rows, n0;
-                walk.seek(tile, e, m0, rows, n0);
-                for (int kb = kb0; kb < kb1; ++kb, ++it) {
-                    const int s = it % S::STAGES;
-                    if (it >= S::STAGES && !mbar_wait(bar_empty(s), ((it / S::STAGES) - 1) & 1, abort_flag, 0x601u)) { ok = false; break; }
+        int s = 0;
+        uint32_t ph = 1;                                   // of bar_empty: the first round finds the stages free
+        bool ok = true;
+        for (int tile = first; tile < tiles && ok; tile += step) {
+            int e, m0, rows, n0;
+            walk.seek(tile, e, m0, rows, n0);
+            for (int kb = kb0; kb < kb1; ++kb) {
+                if (!warp_wait(bar_empty(s), ph, abort_flag, 0x601u)) { ok = false; break; }
+                if (elect_one()) {
                     mbar_expect_tx(bar_full(s), S::STAGE);
                     const int k = kb * BM_BK;
                     tma_load_2d(ROWS_ON_LANES ? l_tile(s) : c_tile(s), &tm_x, bar_full(s), k, m0);
@@ -231,30 +122,37 @@ block_mm_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
                         for (int h = 0; h < S::COL_TILE / 128; ++h) tma_load_3d(wt + h * 16384, &tm_w, bar_full(s), n0 + h * 128, k, e);
                     }
                 }
+                __syncwarp();
+                ++issued;
+                if (++s == S::STAGES) { s = 0; ph ^= 1u; }
             }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            // K-major operands step 32 bytes along the row per K = 32, MN-major ones 32 rows of 128 bytes
-            const uint32_t w_step = p.w_nk ? 32u : 4096u, w_lbo = p.w_nk ? 16u : 16384u;
-            int &it = issued;
-            bool ok = true;
-            for (int tile = first; tile < tiles && ok; tile += step) {
-                for (int kb = kb0; kb < kb1; ++kb, ++it) {
-                    const int s = it % S::STAGES, a = it % S::NBUF;
-                    if (it >= S::NBUF && !mbar_wait(bar_acc_empty(a), ((it / S::NBUF) - 1) & 1, abort_flag, 0x602u)) { ok = false; break; }
-                    if (!mbar_wait(bar_full(s), (it / S::STAGES) & 1, abort_flag, 0x603u)) { ok = false; break; }
-                    tc_fence_after();
-                    const uint32_t d = tmem_base + (uint32_t)(a * NT);
+        // K-major operands step 32 bytes along the row per K = 32, MN-major ones 32 rows of 128 bytes
+        const uint32_t w_step = p.w_nk ? 32u : 4096u, w_lbo = p.w_nk ? 16u : 16384u;
+        const uint64_t x_desc = smem_desc(ROWS_ON_LANES ? l_tile(0) : c_tile(0), 16, 1024), w_desc = smem_desc(ROWS_ON_LANES ? c_tile(0) : l_tile(0), w_lbo, 1024);
+        int s = 0, a = 0;
+        uint32_t ph = 0, aph = 1;
+        bool ok = true;
+        for (int tile = first; tile < tiles && ok; tile += step) {
+            for (int kb = kb0; kb < kb1; ++kb) {
+                if (!warp_wait(bar_acc_empty(a), aph, abort_flag, 0x602u) || !warp_wait(bar_full(s), ph, abort_flag, 0x603u)) { ok = false; break; }
+                tc_fence_after();
+                const uint32_t d = tmem_base + (uint32_t)(a * NT);
+                const uint64_t xd = x_desc + (uint32_t)(s * (S::STAGE >> 4)), wd = w_desc + (uint32_t)(s * (S::STAGE >> 4));
+                if (elect_one()) {
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk) {
-                        const uint64_t xd = smem_desc((ROWS_ON_LANES ? l_tile(s) : c_tile(s)) + kk * 32, 16, 1024);
-                        const uint64_t wd = smem_desc((ROWS_ON_LANES ? c_tile(s) : l_tile(s)) + kk * w_step, w_lbo, 1024);
-                        bm_mma(d, ROWS_ON_LANES ? xd : wd, ROWS_ON_LANES ? wd : xd, idesc, kk > 0 ? 1u : 0u);
+                        const uint64_t xk = xd + (uint32_t)(kk * 2), wk = wd + kk * (w_step >> 4);
+                        bm_mma(d, ROWS_ON_LANES ? xk : wk, ROWS_ON_LANES ? wk : xk, idesc, kk > 0 ? 1u : 0u);
                     }
                     tc_commit(bar_empty(s));
                     tc_commit(bar_acc_full(a));
                 }
+                __syncwarp();
+                ++issued;
+                if (++s == S::STAGES) { s = 0; ph ^= 1u; }
+                if (++a == S::NBUF) { a = 0; aph ^= 1u; }
             }
         }
     } else {
@@ -281,32 +179,42 @@ block_mm_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
                 x_ok[i] = r < rows && (ROWS_ON_LANES || lane + 32 * i < S::COLS);
                 xsp[i] = p.xs + (x_ok[i] ? (int64_t)(m0 + r) * p.nkb : 0);
             }
-            float sw = 0.f, sx[RPL];
-            auto fetch = [&](int kb) {
-                sw = n_ok && kb < kb1 ? __ldg(wsp + (int64_t)kb * ws_step) : 0.f;
+            // fetched two blocks ahead: a miss takes longer than a block
+            float sw[2], sx[2][RPL];
+            auto fetch = [&](int kb, int b) {
+                sw[b] = n_ok && kb < kb1 ? __ldg(wsp + (int64_t)kb * ws_step) : 0.f;
 #pragma unroll
-                for (int i = 0; i < RPL; ++i) sx[i] = x_ok[i] && kb < kb1 ? __ldg(xsp[i] + kb) : 0.f;
+                for (int i = 0; i < RPL; ++i) sx[b][i] = x_ok[i] && kb < kb1 ? __ldg(xsp[i] + kb) : 0.f;
             };
-            fetch(kb0);
+            fetch(kb0, 0);
+            fetch(kb0 + 1, 1);
             uint64_t acc[S::COLS / 2];
 #pragma unroll
             for (int i = 0; i < S::COLS / 2; ++i) acc[i] = 0ull;
             for (int kb = kb0; kb < kb1; ++kb, ++it) {
                 const int a = it % S::NBUF;
-                uint64_t f2 = 0;
+                uint64_t f2 = 0, fv[ROWS_ON_LANES ? 1 : S::COLS / 2];
                 if constexpr (ROWS_ON_LANES) {
-                    const float f = sx[0] * sw;
+                    const float f = sx[0][0] * sw[0];
                     f2 = pack2(__float_as_uint(f), __float_as_uint(f));
                 } else {
                     __syncwarp();
 #pragma unroll
                     for (int i = 0; i < RPL; ++i)
-                        if (lane + 32 * i < S::COLS) fact[lane + 32 * i] = sx[i] * sw;
+                        if (lane + 32 * i < S::COLS) fact[lane + 32 * i] = sx[0][i] * sw[0];
                     __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < S::COLS / 4; ++i) {
+                        const ulonglong2 t = *reinterpret_cast<const ulonglong2 *>(fact + 4 * i);
+                        fv[2 * i] = t.x;
+                        fv[2 * i + 1] = t.y;
+                    }
                 }
-                fetch(kb + 1);
-                // (a vote, so that a wait that gave up takes the whole warp along)
-                if (!__all_sync(0xffffffffu, mbar_wait(bar_acc_full(a), (it / S::NBUF) & 1, abort_flag, 0x604u))) { ok = false; break; }
+                sw[0] = sw[1];
+#pragma unroll
+                for (int i = 0; i < RPL; ++i) sx[0][i] = sx[1][i];
+                fetch(kb + 2, 1);
+                if (!warp_wait(bar_acc_full(a), (it / S::NBUF) & 1, abort_flag, 0x604u)) { ok = false; break; }
                 tc_fence_after();
                 const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(a * NT + set * S::COLS);
                 uint32_t v[2][CH];
@@ -316,16 +224,8 @@ block_mm_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
                     bm_ld_wait<CH>(v[c & 1]);
                     if (c + 1 < NCH) bm_ld<CH>(taddr + (c + 1) * CH, v[(c + 1) & 1]);
 #pragma unroll
-                    for (int i = 0; i < CH; i += 4) {
-                        uint64_t f0 = f2, f1 = f2;
-                        if constexpr (!ROWS_ON_LANES) {
-                            const ulonglong2 fv = *reinterpret_cast<const ulonglong2 *>(fact + c * CH + i);
-                            f0 = fv.x;
-                            f1 = fv.y;
-                        }
-                        fma2(acc[(c * CH + i) / 2], pack2(v[c & 1][i], v[c & 1][i + 1]), f0);
-                        fma2(acc[(c * CH + i) / 2 + 1], pack2(v[c & 1][i + 2], v[c & 1][i + 3]), f1);
-                    }
+                    for (int i = 0; i < CH; i += 2)
+                        fma2(acc[(c * CH + i) / 2], pack2(v[c & 1][i], v[c & 1][i + 1]), ROWS_ON_LANES ? f2 : fv[ROWS_ON_LANES ? 0 : (c * CH + i) / 2]);
                 }
                 tc_fence_before();
                 __syncwarp();
@@ -395,11 +295,22 @@ block_mm_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
                 int e, m0, rows, n0;
                 TileWalk<S::ROW_TILE, S::COL_TILE> w2{row_start, tile_end};
                 w2.seek(first, e, m0, rows, n0);
-                const int t = threadIdx.x - 64, ln = t & 127, n = n0 + ln;
-                for (int r = (t >> 7) * p.split + rank; r < rows; r += S::SETS * p.split) {
-                    float v = 0.f;
-                    for (int c = 0; c < p.split; ++c) v += ld_cluster_f32(base + (uint32_t)(r * BM_LANES + ln) * 4u, (uint32_t)c);
-                    if (n < p.N) store_from_float(p.out, p.out_type, (int64_t)(m0 + r) * p.N + n, v);
+                // a warp sums a row: 4 columns a lane, all parts in flight, added in rank order
+                for (int r = (warp - 2) * p.split + rank; r < rows; r += BM_EPI_WARPS * p.split) {
+                    float4 part[8];
+#pragma unroll
+                    for (int c = 0; c < 8; ++c)
+                        if (c < p.split) part[c] = ld_cluster_f32x4(base + (uint32_t)(r * BM_LANES + lane * 4) * 4u, (uint32_t)c);
+                    float4 v = part[0];
+#pragma unroll
+                    for (int c = 1; c < 8; ++c)
+                        if (c < p.split) { v.x += part[c].x; v.y += part[c].y; v.z += part[c].z; v.w += part[c].w; }
+                    const int n = n0 + lane * 4;
+                    const int64_t at = (int64_t)(m0 + r) * p.N + n;
+                    if (n < p.N) store_from_float(p.out, p.out_type, at, v.x);
+                    if (n + 1 < p.N) store_from_float(p.out, p.out_type, at + 1, v.y);
+                    if (n + 2 < p.N) store_from_float(p.out, p.out_type, at + 2, v.z);
+                    if (n + 3 < p.N) store_from_float(p.out, p.out_type, at + 3, v.w);
                 }
             }
             bm_cluster_sync();                            // a CTA's shared memory outlives the others' reads
@@ -419,16 +330,6 @@ block_mm_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
         tc_fence_after();
         tmem_dealloc(tmem_base, S::TMEM_COLS);
     }
-}
-
-// 3-D map of E matrices of `rows` rows of `cols` bytes.
-bool make_map3(CUtensorMap *tm, const void *ptr, uint64_t cols, uint64_t rows, uint64_t E, uint32_t box_cols, uint32_t box_rows) {
-    EncodeFn fn = encode_fn();
-    if (!fn) return false;
-    cuuint64_t dims[3] = {cols, rows, E}, strides[2] = {cols, cols * rows};
-    cuuint32_t box[3] = {box_cols, box_rows, 1}, estr[3] = {1, 1, 1};
-    return fn(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void *>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <bool ROWS_ON_LANES, int NT> cudaError_t launch_form(const BlockMmArgs &a, int split, cudaStream_t s) {
@@ -467,7 +368,7 @@ bool block_mm_tc_supported(const BlockMmArgs &a) {
 
 cudaError_t launch_block_mm_tc(const BlockMmArgs &a, cudaStream_t s) {
     const int64_t rows = a.experts > 0 ? (a.M + a.experts - 1) / a.experts : a.M;   // of an expert, on average
-    if (rows > 128) return launch_form<true, 256>(a, 1, s);
+    if (rows > 128) return getenv("BM_SINGLE") ? launch_form<true, 256>(a, 1, s) : launch_block_mm_pair(a, s);
     const int nt = rows <= 8 ? 16 : (rows <= 24 ? 32 : (rows <= 56 ? 64 : 128));
     const int64_t nkb = (a.K + BM_BK - 1) / BM_BK, cols = (a.N + 127) / 128, full = (a.M + nt - 1) / nt;
     const int64_t tiles = (a.experts > 0 ? std::min<int64_t>(a.M, full + a.experts - 1) : full) * cols;
@@ -484,11 +385,12 @@ cudaError_t launch_block_mm_tc(const BlockMmArgs &a, cudaStream_t s) {
 unsigned int block_mm_device_status() {
     unsigned int v = 0;
     if (cudaMemcpyFromSymbol(&v, g_tc_status, sizeof(v)) != cudaSuccess) return 0xFFFFFFFFu;
-    return v;
+    return v ? v : block_mm_pair_device_status();
 }
 void block_mm_device_status_reset() {
     const unsigned int z = 0;
     cudaMemcpyToSymbol(g_tc_status, &z, sizeof(z));
+    block_mm_pair_device_status_reset();
 }
 
 }  // namespace qmm

@@ -158,6 +158,10 @@ bool block_mm_tc_supported(const BlockMmArgs &p);
 cudaError_t launch_block_mm_tc(const BlockMmArgs &p, cudaStream_t s);
 unsigned int block_mm_device_status();
 void block_mm_device_status_reset();
+// The same for many rows: pairs of CTAs (block_mm_pair.cu).
+cudaError_t launch_block_mm_pair(const BlockMmArgs &p, cudaStream_t s);
+unsigned int block_mm_pair_device_status();
+void block_mm_pair_device_status_reset();
 
 // Tokens sorted by expert and back (moe_permute.cu).
 constexpr int MOE_MAX_EXPERTS = 1024, MOE_MAX_TOPK = 64;

@@ -5,28 +5,29 @@
 // fetched once thus serves 256 rows and a byte of x 256 columns: 32 KB per CTA and block where a single CTA's 128 x 256 tile needs 48 KB.
 //
 // The block's sums leave tensor memory before the next block's are added (the scales are arbitrary fp32 numbers): two
-// accumulators of 256 columns alternate, and sixteen epilogue warps per CTA fold each into 64 fp32 registers a
+// accumulators of 256 columns alternate, and eight epilogue warps per CTA fold each into 128 fp32 registers a
 // thread, acc += part * (xs[row] * ws[128-column block]), two multiply-adds per instruction.  What bounds the kernel is the
-// round trip of an accumulator -- products, commit, fold, hand-back across the pair, next products -- hence many epilogue warps
-// with a short fold each, scales that are there before the block, and a hand-back before the last multiply-adds.
+// round trip of an accumulator -- products, commit, fold, hand-back across the pair, next products -- hence
+// scales that are there before the block, and a hand-back before the last multiply-adds.  (Sixteen warps with half the columns
+// each fold sooner but issue more: 143 instructions a warp and block, 570 a scheduler against 512 cycles of products.)
 //
 // Roles per CTA: warp 0 = TMA producer of its own halves; warp 1 = in the leader the MMA issuer, in the other CTA the relay
-// that tells the leader its stage is filled; warp 2 = scales; warps 4-19 = epilogue.  Waits are bounded, and the pair meets at a cluster
+// that tells the leader its stage is filled; warp 2 = scales; warps 4-11 = epilogue.  Waits are bounded, and the pair meets at a cluster
 // barrier before either CTA's memory goes away.
 #include "block_mm_common.cuh"
 
 namespace qmm {
 namespace {
 
-constexpr int BP_STAGES = 5, BP_NBUF = 2, BP_ROWS = 256, BP_COLS = 256, BP_EPI = 16, BP_THREADS = 128 + BP_EPI * 32;
+constexpr int BP_STAGES = 5, BP_NBUF = 2, BP_ROWS = 256, BP_COLS = 256, BP_EPI = 8, BP_THREADS = 128 + BP_EPI * 32;
 struct BpSmem {
     static constexpr int X_BYTES = 128 * BM_BK, W_BYTES = 128 * BM_BK, STAGE = X_BYTES + W_BYTES;
     static constexpr int TABLE_OFF = BP_STAGES * STAGE;
-    static constexpr int OUT_OFF = TABLE_OFF + BM_TABLE_BYTES;      // 32 rows x 64 bytes per epilogue warp
-    static constexpr int SC_OFF = OUT_OFF + BP_EPI * 2048;          // per slot: 128 row scales, 2 of the weight's blocks
+    static constexpr int OUT_OFF = TABLE_OFF + BM_TABLE_BYTES;      // 32 rows x 128 bytes per epilogue warp
+    static constexpr int SC_OFF = OUT_OFF + BP_EPI * 4096;          // per slot: 128 row scales, 2 of the weight's blocks
     static constexpr int SC_SLOT = 130 * 4;
     static constexpr int BAR_OFF = (SC_OFF + SC_SLOTS * SC_SLOT + 7) / 8 * 8;
-    static constexpr int NUM_BARS = 2 * BP_STAGES + 2 * BP_NBUF;
+    static constexpr int NUM_BARS = 2 * BP_STAGES + 4 * BP_NBUF;
     static constexpr int MISC_OFF = BAR_OFF + NUM_BARS * 8;
     static constexpr int TOTAL = MISC_OFF + 16 + 1024;
 };
@@ -54,6 +55,46 @@ __device__ __forceinline__ void bp_arrive(uint32_t cluster_bar) {
     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
 
+// A warp's 32 rows x 2 x 64 columns, 128 apart (a row per lane), to global memory, 128 bytes of each row at a time through shared memory,
+// so that a store covers 4 rows and not 32.  Units of 16 bytes; their order in a row is turned by the row so that neither
+// side meets in a bank.  `rows` and `cols` are what is left of the matrix, cols a multiple of 8.
+template <int T, typename E>
+__device__ __forceinline__ void store_rows(const uint64_t (&acc)[64], uint4 *box, E *out, int rows, int cols, int N) {
+    constexpr int UNIT = 16 / (int)sizeof(E), PER = 8 * UNIT, PASSES = 128 / PER;
+    const int lane = threadIdx.x & 31, r0 = lane >> 3, c0 = (lane & 7) * UNIT;
+    E *o = out + (int64_t)r0 * N + c0;
+#pragma unroll
+    for (int pass = 0; pass < PASSES; ++pass) {
+        __syncwarp();
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            uint32_t h[4];
+            if constexpr (T == ET_F32) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) { h[2 * i] = (uint32_t)acc[pass * 16 + 2 * u + i]; h[2 * i + 1] = (uint32_t)(acc[pass * 16 + 2 * u + i] >> 32); }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float f0, f1;
+                    unpack2(acc[pass * 32 + 4 * u + i], f0, f1);
+                    if constexpr (T == ET_BF16) { __nv_bfloat162 b = __floats2bfloat162_rn(f0, f1); h[i] = *reinterpret_cast<uint32_t *>(&b); }
+                    else { __half2 b = __floats2half2_rn(f0, f1); h[i] = *reinterpret_cast<uint32_t *>(&b); }
+                }
+            }
+            box[lane * 8 + (u ^ (lane & 7))] = make_uint4(h[0], h[1], h[2], h[3]);
+        }
+        __syncwarp();
+        const int c = pass * PER + (pass >= PASSES / 2 ? 64 : 0);
+        if (c + c0 < cols) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int r = i * 4 + r0;
+                if (r < rows) *reinterpret_cast<uint4 *>(o + (int64_t)(i * 4) * N + c) = box[r * 8 + ((lane & 7) ^ (r & 7))];
+            }
+        }
+    }
+}
+
 __global__ void __launch_bounds__(BP_THREADS, 1)
 block_mm_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w, const BmParams p, const uint32_t idesc) {
     using S = BpSmem;
@@ -64,8 +105,9 @@ block_mm_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
     auto w_tile = [&](int s) { return base + s * S::STAGE + S::X_BYTES; };
     auto bar_full = [&](int s) { return base + S::BAR_OFF + 8 * s; };        // in the leader: of both CTAs' stages
     auto bar_empty = [&](int s) { return base + S::BAR_OFF + 8 * (BP_STAGES + s); };
-    auto bar_acc_full = [&](int a) { return base + S::BAR_OFF + 8 * (2 * BP_STAGES + a); };              // products and scales
-    auto bar_acc_empty = [&](int a) { return base + S::BAR_OFF + 8 * (2 * BP_STAGES + BP_NBUF + a); };   // leader: both CTAs' epilogues
+    // accumulator a (alternating) of half h
+    auto bar_acc_full = [&](int h, int a) { return base + S::BAR_OFF + 8 * (2 * BP_STAGES + h * BP_NBUF + a); };            // products and scales
+    auto bar_acc_empty = [&](int h, int a) { return base + S::BAR_OFF + 8 * (2 * BP_STAGES + (2 + h) * BP_NBUF + a); };     // leader: both CTAs' epilogues
     int *row_start = reinterpret_cast<int *>(gen_base + S::TABLE_OFF), *tile_end = row_start + p.E + 1;
     volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(gen_base + S::MISC_OFF);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(gen_base + S::MISC_OFF + 4);
@@ -73,8 +115,9 @@ block_mm_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
     const int rank = (int)blockIdx.x & 1;
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < BP_STAGES; ++s) { mbar_init(bar_full(s), rank == 0 ? 2 : 1); mbar_init(bar_empty(s), 1); }
-        for (int a = 0; a < BP_NBUF; ++a) { mbar_init(bar_acc_full(a), 2); mbar_init(bar_acc_empty(a), 2 * BP_EPI); }
+        for (int s = 0; s < BP_STAGES; ++s) { mbar_init(bar_full(s), rank == 0 ? 2 : 1); mbar_init(bar_empty(s), 2); }
+        for (int h = 0; h < 2; ++h)
+            for (int a = 0; a < BP_NBUF; ++a) { mbar_init(bar_acc_full(h, a), 2); mbar_init(bar_acc_empty(h, a), BP_EPI); }
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_proxy_async();
@@ -93,8 +136,12 @@ block_mm_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
     const int tiles = tile_end[p.E - 1];
     const int first = (int)blockIdx.x >> 1, step = (int)gridDim.x >> 1;
     TileWalk<BP_ROWS, BP_COLS> walk{row_start, tile_end};
+    // The epilogue needs 128 sums and two loads of 32 in registers: the first four warps give up what they do not use.
+    // (384 threads x 168 at launch = 128 x 56 + 256 x 224.)
     int issued = 0;                                       // warp 0: stages filled; the leader's warp 1: blocks multiplied
 
+    if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 0) {
         int s = 0;
         uint32_t ph = 1;                                  // of bar_empty: the first round finds the stages free
@@ -117,38 +164,42 @@ block_mm_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
                 if (++s == BP_STAGES) { s = 0; ph ^= 1u; }
             }
         }
-    } else if (warp == 1) {
-        const uint32_t w_step = p.w_nk ? 32u : 4096u, w_lbo = p.w_nk ? 16u : 16384u;
-        const uint64_t x_desc = smem_desc(x_tile(0), 16, 1024), w_desc = smem_desc(w_tile(0), w_lbo, 1024);
+    } else if (warp == 1 || warp == 3) {
+        // The leader's two issuers, one per half: 64 of the weight columns of each CTA, 64 rows of 128 bytes or 64 bytes of each row
+        // apart.  In the other CTA warp 1 reports filled stages to the leader.
+        const int h = warp >> 1;
+        const uint32_t w_step = p.w_nk ? 32u : 4096u, w_lbo = p.w_nk ? 16u : 16384u, w_half = p.w_nk ? 8192u : 64u;
+        const uint64_t x_desc = smem_desc(x_tile(0), 16, 1024), w_desc = smem_desc(w_tile(0) + (uint32_t)h * w_half, w_lbo, 1024);
+        const uint32_t peer_full = bp_at(bar_full(0), 0);
         int s = 0, a = 0;
         uint32_t ph = 0, aph = 1;
         bool ok = true;
         for (int tile = first; tile < tiles && ok; tile += step) {
             for (int kb = 0; kb < p.nkb; ++kb) {
                 if (rank == 0) {
-                    if (!warp_wait<true>(bar_full(s), ph, abort_flag, 0x613u) || !warp_wait<true>(bar_acc_empty(a), aph, abort_flag, 0x612u)) { ok = false; break; }
+                    if (!warp_wait<true>(bar_full(s), ph, abort_flag, 0x613u) || !warp_wait<true>(bar_acc_empty(h, a), aph, abort_flag, 0x612u)) { ok = false; break; }
                     tc_fence_after();
-                    const uint32_t d = tmem_base + (uint32_t)(a * BP_COLS);
+                    const uint32_t d = tmem_base + (uint32_t)(a * BP_COLS + h * 128);
                     const uint64_t xd = x_desc + (uint32_t)(s * (S::STAGE >> 4)), wd = w_desc + (uint32_t)(s * (S::STAGE >> 4));
                     if (elect_one()) {
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk) bp_mma(d, xd + (uint32_t)(kk * 2), wd + kk * (w_step >> 4), idesc, kk > 0 ? 1u : 0u);
-                        bp_commit(bar_acc_full(a));
+                        bp_commit(bar_acc_full(h, a));
                         bp_commit(bar_empty(s));
                     }
                     __syncwarp();
                     ++issued;
                     a ^= 1;
                     if (a == 0) aph ^= 1u;
-                } else {
+                } else if (h == 0) {
                     if (!warp_wait(bar_full(s), ph, abort_flag, 0x615u)) { ok = false; break; }
-                    if (elect_one()) bp_arrive(bp_at(bar_full(s), 0));
+                    if (elect_one()) bp_arrive(peer_full + 8u * (uint32_t)s);
                     __syncwarp();
                 }
                 if (++s == BP_STAGES) { s = 0; ph ^= 1u; }
             }
         }
-    } else if (warp == 2) {
+    } else {
         // scales: the copies run SC_AHEAD blocks in front of the reports.  Slots are reused 16 blocks later, and a report
         // for block i waits for block i - 2 to be complete, by when block i - 4 has been folded.
         TileWalk<BP_ROWS, BP_COLS> ahead{row_start, tile_end};
@@ -184,21 +235,23 @@ block_mm_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
         bool ok = true;
         for (int tile = first; tile < tiles && ok; tile += step) {
             for (int kb = 0; kb < p.nkb; ++kb) {
-                if (!warp_wait(bar_acc_full(a), ph, abort_flag, 0x617u)) { ok = false; break; }
+                if (!warp_wait(bar_acc_full(0, a), ph, abort_flag, 0x617u) || !warp_wait(bar_acc_full(1, a), ph, abort_flag, 0x618u)) { ok = false; break; }
                 copy_next();
                 cp_async_wait<SC_AHEAD>();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(bar_acc_full(a));
+                if (lane < 2) mbar_arrive(bar_acc_full(lane, a));
                 a ^= 1;
                 if (a == 0) ph ^= 1u;
             }
         }
         cp_async_wait<0>();
-    } else if (warp >= 4) {
-        const int ew = warp - 4, set = ew >> 2, q = warp & 3;
-        constexpr int COLS = BP_COLS / 4, CH = 16, NCH = COLS / CH;
-        const uint32_t tm_lane = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(set * COLS);
-        const uint32_t give = bp_at(bar_acc_empty(0), 0);  // in the leader, of accumulator 0; 8 bytes on, of 1
+    }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        const int ew = warp - 4, h = ew >> 2, q = warp & 3;   // h: this warp's half
+        constexpr int COLS = BP_COLS / 2, CH = 32, NCH = COLS / CH;
+        const uint32_t tm_lane = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(h * COLS);
+        const uint32_t give = bp_at(bar_acc_empty(h, 0), 0);   // in the leader, of accumulator 0; 8 bytes on, of 1
         int a = 0, slot = 0;
         uint32_t ph = 0;
         bool ok = true;
@@ -207,25 +260,27 @@ block_mm_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
 #pragma unroll
             for (int i = 0; i < COLS / 2; ++i) acc[i] = 0ull;
             for (int kb = 0; kb < p.nkb; ++kb) {
-                if (!warp_wait(bar_acc_full(a), ph, abort_flag, 0x616u)) { ok = false; break; }
+                if (!warp_wait(bar_acc_full(h, a), ph, abort_flag, 0x616u)) { ok = false; break; }
                 tc_fence_after();
                 const uint32_t taddr = tm_lane + (uint32_t)(a * BP_COLS);
-                uint32_t v[CH];
-                bm_ld<CH>(taddr, v);
+                uint32_t v[2][CH];
+                bm_ld<CH>(taddr, v[0]);
                 const float *sc = reinterpret_cast<const float *>(gen_base + S::SC_OFF + slot * S::SC_SLOT);
-                const float f = sc[q * 32 + lane] * sc[128 + (set >> 1)];
-                const uint64_t f2 = pack2(__float_as_uint(f), __float_as_uint(f));
+                // the half's first 64 columns lie in the tile's first 128 (the leader's), the others in the second
+                const float sx = sc[q * 32 + lane], f0 = sx * sc[128], f1 = sx * sc[129];
+                const uint64_t f2[2] = {pack2(__float_as_uint(f0), __float_as_uint(f0)), pack2(__float_as_uint(f1), __float_as_uint(f1))};
 #pragma unroll
                 for (int c = 0; c < NCH; ++c) {
-                    bm_ld_wait<CH>(v);
-                    if (c + 1 == NCH) {                   // all of it is in registers: the accumulator is free
+                    bm_ld_wait<CH>(v[c & 1]);
+                    if (c + 1 < NCH) {
+                        bm_ld<CH>(taddr + (c + 1) * CH, v[(c + 1) & 1]);
+                    } else {                              // all of it is in registers: the accumulator is free
                         tc_fence_before();
                         __syncwarp();
                         if (lane == 0) bp_arrive(give + 8u * (uint32_t)a);
                     }
 #pragma unroll
-                    for (int i = 0; i < CH; i += 2) fma2(acc[(c * CH + i) / 2], pack2(v[i], v[i + 1]), f2);
-                    if (c + 1 < NCH) bm_ld<CH>(taddr + (c + 1) * CH, v);
+                    for (int i = 0; i < CH; i += 2) fma2(acc[(c * CH + i) / 2], pack2(v[c & 1][i], v[c & 1][i + 1]), f2[2 * c / NCH]);
                 }
                 slot = (slot + 1) & (SC_SLOTS - 1);
                 a ^= 1;
@@ -236,54 +291,22 @@ block_mm_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
             walk.seek(tile, e, m0, rows, n0);
             m0 += rank * 128 + q * 32;                    // this warp's rows
             rows -= rank * 128 + q * 32;
-            const int nc = n0 + set * COLS;
+            const int nc = n0 + h * 64;                   // and 128 further on
             if (p.vec_out) {                              // N a multiple of 8, 16-byte aligned
-                // 64 bytes of each row at a time through shared memory, so that a store covers 8 rows and not 32
-                // (units of 16 bytes, their order in a row turned by the row so that neither side meets in a bank)
-                const bool f32 = p.out_type == ET_F32;
-                const int per = f32 ? 16 : 32, unit = f32 ? 4 : 8;    // columns of a pass, of 16 bytes
-                uint4 *box = reinterpret_cast<uint4 *>(gen_base + S::OUT_OFF) + ew * 128;
-#pragma unroll
-                for (int pass = 0; pass < 4; ++pass) {
-                    if (pass >= 2 && !f32) break;
-                    __syncwarp();
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        uint4 w;
-                        if (f32) {
-                            const uint64_t w0 = acc[pass * 8 + 2 * u], w1 = acc[pass * 8 + 2 * u + 1];
-                            w = make_uint4((uint32_t)w0, (uint32_t)(w0 >> 32), (uint32_t)w1, (uint32_t)(w1 >> 32));
-                        } else {
-                            uint32_t h[4];
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                float f0, f1;
-                                unpack2(acc[(pass & 1) * 16 + 4 * u + i], f0, f1);
-                                if (p.out_type == ET_BF16) { __nv_bfloat162 b = __floats2bfloat162_rn(f0, f1); h[i] = *reinterpret_cast<uint32_t *>(&b); }
-                                else { __half2 b = __floats2half2_rn(f0, f1); h[i] = *reinterpret_cast<uint32_t *>(&b); }
-                            }
-                            w = make_uint4(h[0], h[1], h[2], h[3]);
-                        }
-                        box[lane * 4 + (u ^ ((lane >> 1) & 3))] = w;
-                    }
-                    __syncwarp();
-                    const int col = nc + pass * per + (lane & 3) * unit;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int r = i * 8 + (lane >> 2);
-                        const uint4 t = box[r * 4 + ((lane & 3) ^ ((r >> 1) & 3))];
-                        if (r < rows && col < p.N)
-                            *reinterpret_cast<uint4 *>((uint8_t *)p.out + ((int64_t)(m0 + r) * p.N + col) * (f32 ? 4 : 2)) = t;
-                    }
-                }
+                uint4 *box = reinterpret_cast<uint4 *>(gen_base + S::OUT_OFF) + ew * 256;
+                const int64_t at = (int64_t)m0 * p.N + nc;
+                if (p.out_type == ET_BF16) store_rows<ET_BF16>(acc, box, (uint16_t *)p.out + at, rows, p.N - nc, p.N);
+                else if (p.out_type == ET_F16) store_rows<ET_F16>(acc, box, (uint16_t *)p.out + at, rows, p.N - nc, p.N);
+                else store_rows<ET_F32>(acc, box, (float *)p.out + at, rows, p.N - nc, p.N);
             } else if (lane < rows) {
                 const int64_t at = (int64_t)(m0 + lane) * p.N + nc;
 #pragma unroll
                 for (int i = 0; i < COLS / 2; ++i) {
                     float f0, f1;
                     unpack2(acc[i], f0, f1);
-                    if (nc + 2 * i < p.N) store_from_float(p.out, p.out_type, at + 2 * i, f0);
-                    if (nc + 2 * i + 1 < p.N) store_from_float(p.out, p.out_type, at + 2 * i + 1, f1);
+                    const int c = 2 * i + (i >= COLS / 4 ? 64 : 0);
+                    if (nc + c < p.N) store_from_float(p.out, p.out_type, at + c, f0);
+                    if (nc + c + 1 < p.N) store_from_float(p.out, p.out_type, at + c + 1, f1);
                 }
             }
             __syncwarp();
@@ -296,8 +319,8 @@ block_mm_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
         // a wait gave up: copies and products in flight end before the pair's memory goes (each awaited with a limit)
         if (warp == 0 && lane == 0)
             for (int j = issued > BP_STAGES ? issued - BP_STAGES : 0; j < issued; ++j) bm_drain(bar_full(j % BP_STAGES), (j / BP_STAGES) & 1);
-        if (warp == 1 && lane == 0)
-            for (int j = issued > BP_NBUF ? issued - BP_NBUF : 0; j < issued; ++j) bm_drain(bar_acc_full(j % BP_NBUF), (j / BP_NBUF) & 1);
+        if ((warp == 1 || warp == 3) && lane == 0)
+            for (int j = issued > BP_NBUF ? issued - BP_NBUF : 0; j < issued; ++j) bm_drain(bar_acc_full(warp >> 1, j % BP_NBUF), (j / BP_NBUF) & 1);
     }
     bm_cluster_sync();
     if (warp == 1) {
@@ -319,7 +342,7 @@ cudaError_t launch_block_mm_pair(const BlockMmArgs &a, cudaStream_t s) {
     p.vec_out = a.N % 8 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
     p.M = (int)a.M; p.N = (int)a.N; p.nkb = (int)((a.K + BM_BK - 1) / BM_BK); p.nb = (int)((a.N + 127) / 128); p.E = E;
     p.n_tiles = (int)((a.N + BP_COLS - 1) / BP_COLS); p.w_nk = a.w_nk; p.split = 1;
-    const uint32_t idesc = bm_idesc(a.x_type == ET_E5M2, a.w_type == ET_E5M2, 0, a.w_nk ? 0 : 1, BP_ROWS, BP_COLS);
+    const uint32_t idesc = bm_idesc(a.x_type == ET_E5M2, a.w_type == ET_E5M2, 0, a.w_nk ? 0 : 1, BP_ROWS, BP_COLS / 2);
     // tiles: each expert with rows adds at most one partly filled row tile
     const int64_t full = (a.M + BP_ROWS - 1) / BP_ROWS, most = a.experts > 0 ? (a.M < full + E - 1 ? a.M : full + E - 1) : full;
     const int64_t tiles = most * p.n_tiles, pairs = sm_count() / 2;

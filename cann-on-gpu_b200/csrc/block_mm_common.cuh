@@ -7,7 +7,7 @@
 namespace qmm {
 namespace {
 
-constexpr int BM_LANES = 128, BM_BK = 128, BM_EPI_WARPS = 8, BM_THREADS = 64 + BM_EPI_WARPS * 32;
+constexpr int BM_LANES = 128, BM_BK = 128;
 constexpr int BM_TABLE_BYTES = (2 * BLOCK_MM_MAX_EXPERTS + 4) * 4;   // row starts [E + 1], tile ends [E]
 
 struct BmParams {
@@ -74,6 +74,11 @@ __device__ __forceinline__ void unpack2(uint64_t v, float &lo, float &hi) {
     hi = __uint_as_float(b);
 }
 // Two fp32 fused multiply-adds in one instruction.
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
 __device__ __forceinline__ void fma2(uint64_t &acc, uint64_t a, uint64_t b) { asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(a), "l"(b)); }
 
 // One lane of a converged warp; the compiler keeps the operands of what it guards in uniform registers (a branch on the

@@ -348,6 +348,7 @@ cudaError_t launch_block_mm_pair(const BlockMmArgs &a, cudaStream_t s) {
     const int64_t tiles = most * p.n_tiles, pairs = sm_count() / 2;
     cudaError_t e = allow_smem<block_mm_pair_kernel>(BpSmem::TOTAL);
     if (e != cudaSuccess) return e;
+    if (!has_regs<block_mm_pair_kernel>(168)) return cudaErrorInvalidConfiguration;
     e = launch_chained(block_mm_pair_kernel, 2 * (unsigned)(tiles < pairs ? tiles : pairs), BP_THREADS, BpSmem::TOTAL, 2, s, tx, tw, p, idesc);
     if (e == cudaSuccess) count_launch();
     return e;

@@ -30,6 +30,19 @@ template <auto Kernel> cudaError_t allow_smem(int bytes) {
     if (e == cudaSuccess) done[dev].store(true, std::memory_order_release);
     return e;
 }
+// Whether `Kernel` was built for `regs` registers a thread: kernels that move registers between their warps (setmaxnreg) wait
+// for ever when the launch does not have what they share out.
+template <auto Kernel> bool has_regs(int regs) {
+    static std::atomic<int> known;
+    int n = known.load(std::memory_order_relaxed);
+    if (n == 0) {
+        cudaFuncAttributes a;
+        if (cudaFuncGetAttributes(&a, Kernel) != cudaSuccess) return false;
+        n = a.numRegs;
+        known.store(n, std::memory_order_relaxed);
+    }
+    return n == regs;
+}
 // Launch that may start while the kernel before it on the stream drains (the kernel waits with griddepcontrol.wait
 // before it touches global memory), as clusters of `cluster` CTAs.
 template <typename... P, typename... A>

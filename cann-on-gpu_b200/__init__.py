@@ -302,14 +302,13 @@ def cast(src, src_kind, dst_kind, n, **kw):
 # ---------------------------------------------------------------- the expert layer: fp8 with a scale per 128 (aclnn_block_quant_moe.h)
 class _Call:
     """One operator at one set of shapes and types: its aclTensor handles and prepared phase arguments.  A handle is
-    metadata only: every call points it at its own tensors first (aclSetRawTensorAddr), so nothing of a call's data is kept."""
+    metadata only: every call points it at its own tensors first, so nothing of a call's data is kept."""
 
     def __init__(self, lib, name, args):
         import torch
         self.lib, self.handles = lib, []
         self.phase1, self.phase2 = getattr(lib, name + "GetWorkspaceSize"), getattr(lib, name)
-        self.set_addr = lib.aclSetRawTensorAddr
-        self.set_addr.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
+        self.set_addrs = lib.aclnnB200SetRawTensorAddrs
         self.ws, self.ex = ctypes.c_uint64(0), ctypes.c_void_p(0)
         self.ws_ptr, self.ws_size, self.stream = ctypes.c_void_p(0), ctypes.c_uint64(0), ctypes.c_void_p(0)
         self.args = []
@@ -324,6 +323,9 @@ class _Call:
             else:
                 self.args.append(None if a is None else (ctypes.c_bool(a) if isinstance(a, bool) else ctypes.c_int64(a)))
         self.args += [ctypes.byref(self.ws), ctypes.byref(self.ex)]
+        n = len(self.handles)
+        self.addrs = (ctypes.c_void_p * n)()
+        self.addr_args = ((ctypes.c_void_p * n)(*self.handles), self.addrs, ctypes.c_uint64(n))
 
     def __del__(self):
         try:
@@ -331,6 +333,20 @@ class _Call:
                 self.lib.aclDestroyTensor(ctypes.c_void_p(h))
         except Exception:
             pass
+
+
+_current_fns = None
+
+
+def _current(torch):
+    """(current device, current stream of a device as a number): torch's own raw getters where it has them, which take a
+    tenth of the public ones' time on a path whose kernels run for a few microseconds."""
+    global _current_fns
+    if _current_fns is None:
+        torch.cuda.current_device()   # sets CUDA up
+        raw_dev, raw_stream = getattr(torch._C, "_cuda_getDevice", None), getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        _current_fns = (raw_dev or torch.cuda.current_device, raw_stream or (lambda dev: torch.cuda.current_stream(dev).cuda_stream))
+    return _current_fns
 
 
 class _Calls(threading.local):   # a set of handles serves one call at a time: each thread has its own
@@ -365,7 +381,7 @@ def _run(name, *args, stream=None, return_status=False):
             key.append(a.dtype)
         else:
             key.append(a)
-    if dev != torch.cuda.current_device():
+    if dev != _current(torch)[0]():
         with torch.cuda.device(dev):
             return _run(name, *args, stream=stream, return_status=return_status)
     key, known = tuple(key), _calls.known
@@ -374,15 +390,14 @@ def _run(name, *args, stream=None, return_status=False):
         if len(known) >= _calls.MOST:
             known.clear()
         c = known[key] = _Call(lib, name, args)
-    set_addr = c.set_addr
-    for h, t in zip(c.handles, tensors):
-        set_addr(h, t.data_ptr())
+    c.addrs[:] = [t.data_ptr() for t in tensors]
+    c.set_addrs(*c.addr_args)
     st = c.phase1(*c.args)
     if st == ACLNN_SUCCESS:
         need = c.ws.value
         ws = torch.empty(need, dtype=torch.uint8, device=tensors[0].device) if need else None
         c.ws_ptr.value, c.ws_size.value = ws.data_ptr() if need else None, need
-        c.stream.value = torch.cuda.current_stream(dev).cuda_stream if stream is None else stream
+        c.stream.value = _current(torch)[1](dev) if stream is None else stream
         st = c.phase2(c.ws_ptr, c.ws_size, c.ex, c.stream)
     if return_status:
         return st

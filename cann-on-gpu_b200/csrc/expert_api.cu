@@ -267,4 +267,12 @@ aclnnStatus aclnnB200MoeTokenUnpermuteGradGetWorkspaceSize(const aclTensor *grad
 }
 RUN_EXPERT(aclnnB200MoeTokenUnpermuteGrad, PLAN_UNPERMUTE_GRAD)
 
+aclnnStatus aclnnB200SetRawTensorAddrs(aclTensor *const *tensors, void *const *addrs, uint64_t count) {
+    if (count > 0 && (!tensors || !addrs)) return ACLNN_ERR_PARAM_NULLPTR;
+    for (uint64_t i = 0; i < count; ++i)
+        if (!tensors[i]) return ACLNN_ERR_PARAM_NULLPTR;
+    for (uint64_t i = 0; i < count; ++i) tensors[i]->data = addrs[i];
+    return ACLNN_SUCCESS;
+}
+
 }  // extern "C"

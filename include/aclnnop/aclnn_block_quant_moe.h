@@ -102,6 +102,9 @@ ACL_FUNC_VISIBILITY aclnnStatus aclnnB200MoeTokenUnpermuteGradGetWorkspaceSize(c
     uint64_t *workspaceSize, aclOpExecutor **executor);
 B200_ACLNN_RUN(aclnnB200MoeTokenUnpermuteGrad)
 
+/* aclSetRawTensorAddr for `count` tensors in one call, for callers that keep their tensors between calls. */
+ACL_FUNC_VISIBILITY aclnnStatus aclnnB200SetRawTensorAddrs(aclTensor *const *tensors, void *const *addrs, uint64_t count);
+
 #ifdef __cplusplus
 }
 #endif

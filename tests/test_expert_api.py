@@ -162,6 +162,21 @@ def test_phase2_refuses_before_launching(pkg):
                                                  at([1, 1], F, 0x2000), cbool(False), at([0, 32], B, 0))) == OK
 
 
+def test_set_raw_tensor_addrs(pkg):
+    lib = pkg.load()
+    t = [FakeTensor(pkg, [4], pkg.ACL_FLOAT), FakeTensor(pkg, [5], pkg.ACL_FLOAT)]
+    vp, u64 = ctypes.c_void_p, ctypes.c_uint64
+    hs, addrs = (vp * 2)(t[0].h, t[1].h), (vp * 2)(0x1000, 0x2000)
+    assert lib.aclnnB200SetRawTensorAddrs(hs, addrs, u64(2)) == OK
+    got = vp(0)
+    for x, want in zip(t, (0x1000, 0x2000)):
+        assert lib.aclGetRawTensorAddr(vp(x.h), ctypes.byref(got)) == OK and got.value == want
+    assert lib.aclnnB200SetRawTensorAddrs(None, addrs, u64(2)) == NULL and lib.aclnnB200SetRawTensorAddrs(hs, None, u64(2)) == NULL
+    assert lib.aclnnB200SetRawTensorAddrs((vp * 2)(t[0].h, None), (vp * 2)(0x3000, 0), u64(2)) == NULL
+    assert lib.aclGetRawTensorAddr(vp(t[0].h), ctypes.byref(got)) == OK and got.value == 0x1000      # all or none
+    assert lib.aclnnB200SetRawTensorAddrs(None, None, u64(0)) == OK
+
+
 def test_wrappers_refuse_what_the_abi_would_misread(pkg):
     import torch
     with pytest.raises(ValueError):

@@ -5,6 +5,8 @@
 
 #include <cuda_runtime.h>
 
+#include "kernels.h"
+
 namespace qmm {
 
 inline int current_device() {
@@ -62,6 +64,23 @@ cudaError_t launch_chained(void (*kernel)(P...), unsigned grid, unsigned threads
     cfg.attrs = attr;
     cfg.numAttrs = cluster > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+
+// Launch of a kernel whose CTAs step through `work` items: as many as stay resident, at most one per item.
+template <auto Kernel, typename... A> cudaError_t launch_resident(int64_t work, int threads, cudaStream_t s, A... args) {
+    static std::atomic<int> known[64][8];   // CTAs per SM by device and warps
+    const int dev = current_device(), slot = threads / 32 - 1;
+    int per_sm = slot < 8 ? known[dev][slot].load(std::memory_order_relaxed) : 0;
+    if (per_sm == 0) {
+        const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, Kernel, threads, 0);
+        if (e != cudaSuccess) return e;
+        if (per_sm < 1) return cudaErrorLaunchOutOfResources;
+        if (slot < 8) known[dev][slot].store(per_sm, std::memory_order_relaxed);
+    }
+    const int64_t most = (int64_t)per_sm * sm_count();
+    Kernel<<<(unsigned)(work < most ? work : most), threads, 0, s>>>(args...);
+    count_launch();
+    return cudaGetLastError();
 }
 
 }  // namespace qmm

@@ -34,27 +34,41 @@ __device__ __forceinline__ int ld_remote(const int *local, int cta) {
     return v;
 }
 
+// (Eight ids of a lane are loaded at once: one at a time, 65536 pairs took 22 us, two thirds of it load latency.)
+constexpr int SORT_RUN = 8;
 __global__ void __cluster_dims__(SORT_CTAS, 1, 1) __launch_bounds__(SORT_WARPS * 32)
 moe_sort_kernel(const void *ids, bool ids64, int32_t *place, int64_t *counts, int64_t N, int E) {
-    extern __shared__ int hist[];                 // [SORT_WARPS][E], then [E] totals of the CTA
+    extern __shared__ int hist[];                 // [SORT_WARPS][E], then [E] totals of the CTA, then [E] first places
     __shared__ int scan[32];
-    int *cta_total = hist + SORT_WARPS * E;
+    int *cta_total = hist + SORT_WARPS * E, *start = cta_total + E;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, cta = blockIdx.x;
     int *mine = hist + warp * E;
     for (int i = lane; i < E; i += 32) mine[i] = 0;
     __syncwarp();
     const int64_t share = (N + SORT_CTAS * SORT_WARPS * 32 - 1) / (SORT_CTAS * SORT_WARPS * 32) * 32;
     const int64_t lo = (int64_t)(cta * SORT_WARPS + warp) * share, hi = lo + share < N ? lo + share : N;
-    for (int64_t i0 = lo; i0 < hi; i0 += 32) {
-        const int64_t i = i0 + lane;
-        const int e = i < hi ? expert_of(ids, ids64, i, E) : -1;
-        const unsigned same = __match_any_sync(0xffffffffu, e);
-        if (e >= 0 && (same & ((1u << lane) - 1)) == 0) mine[e] += __popc(same);
-        __syncwarp();
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    int e[SORT_RUN];
+    auto load = [&](int64_t i0) {
+#pragma unroll
+        for (int r = 0; r < SORT_RUN; ++r) {
+            const int64_t i = i0 + 32 * r + lane;
+            e[r] = i < hi ? expert_of(ids, ids64, i, E) : -1;
+        }
+    };
+    for (int64_t i0 = lo; i0 < hi; i0 += 32 * SORT_RUN) {
+        load(i0);
+#pragma unroll
+        for (int r = 0; r < SORT_RUN; ++r) {
+            const unsigned same = __match_any_sync(0xffffffffu, e[r]);
+            if (e[r] >= 0 && (same & ((1u << lane) - 1)) == 0) mine[e[r]] += __popc(same);
+            __syncwarp();
+        }
     }
     __syncthreads();
     if (tid < E) {
         int run = 0;
+#pragma unroll
         for (int w = 0; w < SORT_WARPS; ++w) {
             const int c = hist[w * E + tid];
             hist[w * E + tid] = run;
@@ -85,20 +99,23 @@ moe_sort_kernel(const void *ids, bool ids64, int32_t *place, int64_t *counts, in
     int base = incl - total + before;
     for (int w = 0; w < warp; ++w) base += scan[w];
     if (tid < E) {
-        for (int w = 0; w < SORT_WARPS; ++w) hist[w * E + tid] += base;
+        start[tid] = base;
         if (cta == 0) counts[tid] = total;
     }
     __syncthreads();
-    for (int64_t i0 = lo; i0 < hi; i0 += 32) {
-        const int64_t i = i0 + lane;
-        const int e = i < hi ? expert_of(ids, ids64, i, E) : -1;
-        const unsigned same = __match_any_sync(0xffffffffu, e);
-        const unsigned below = same & ((1u << lane) - 1);
-        const int at = e >= 0 ? mine[e] + __popc(below) : -1;
-        __syncwarp();
-        if (e >= 0 && below == 0) mine[e] += __popc(same);
-        __syncwarp();
-        if (i < hi) place[i] = at;
+    for (int64_t i0 = lo; i0 < hi; i0 += 32 * SORT_RUN) {
+        if (share > 32 * SORT_RUN) load(i0);      // a single run is still in registers
+#pragma unroll
+        for (int r = 0; r < SORT_RUN; ++r) {
+            const int64_t i = i0 + 32 * r + lane;
+            const unsigned same = __match_any_sync(0xffffffffu, e[r]);
+            const unsigned below = same & ((1u << lane) - 1);
+            const int at = e[r] >= 0 ? start[e[r]] + mine[e[r]] + __popc(below) : -1;
+            __syncwarp();
+            if (e[r] >= 0 && below == 0) mine[e[r]] += __popc(same);
+            __syncwarp();
+            if (i < hi) place[i] = at;
+        }
     }
     cluster_wait();
 }
@@ -117,7 +134,9 @@ __global__ void __launch_bounds__(256) moe_scatter_kernel(const U *tokens, const
 #pragma unroll
     for (int i = 0; i < 4; ++i)
         if (u0 + 32 * i < units) v[i] = __ldg(tokens + t * units + u0 + 32 * i);
-    const int32_t p0 = lane < k ? __ldg(place + t * k + lane) : -1, p1 = lane + 32 < k ? __ldg(place + t * k + lane + 32) : -1;
+    // launched while the sort runs: the tokens are the caller's, ready before it, but the places and the rows are not
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int32_t p0 = lane < k ? place[t * k + lane] : -1, p1 = lane + 32 < k ? place[t * k + lane + 32] : -1;
     for (int j = 0; j < k; ++j) {
         const int64_t r = __shfl_sync(0xffffffffu, j < 32 ? p0 : p1, j & 31);
         if (r < 0) continue;
@@ -242,120 +261,197 @@ template <int T, bool VEC> struct RowPiece {
 };
 
 // ---- weighted sum of a token's rows --------------------------------------------------------------
-// A warp takes 32 x 16 bytes of one token's output and sums them over the token's rows, GATHER_J rows in flight.
-constexpr int GATHER_J = 8;
-template <int T, bool VEC>
-__global__ void __launch_bounds__(256) moe_gather_kernel(const void *rows, const int32_t *place, const void *probs, int probs_type, void *out,
-                                                         int64_t n_tokens, int k, int64_t R, int64_t H, int64_t segs) {
-    using P = RowPiece<T, VEC>;
-    const int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+// A warp takes 32 x B bytes of one token's output and sums them over the token's rows, J rows in flight.  The warps stay
+// and step through (token, piece), the next token's places and weights on their way while this one's rows are.
+// Bound by HBM reads, so little else may be done per byte: with 16 bytes a lane, a branch per row and 64-bit products for the
+// addresses the issue slots were half full and 8191 x 8 rows of 4096 bf16 took 123-131 us (floor 93).
+template <int B> __device__ __forceinline__ void load_bytes(const char *p, uint32_t (&w)[B / 4]) {
+    if constexpr (B == 32)
+        asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7]) : "l"(p));
+    else {
+        const uint4 v = __ldg(reinterpret_cast<const uint4 *>(p));
+        w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+    }
+}
+template <int T, int B, int J>
+__global__ void __launch_bounds__(256) moe_gather_kernel(const char *rows, const int32_t *place, const void *probs, int probs_type, char *out,
+                                                         int64_t n_tokens, int k, int64_t R, uint32_t pitch, int segs) {
+    constexpr int W = B / 4, PAIRS = T == ET_F32 ? W / 2 : W;     // words of a lane's piece, pairs of values
     const int lane = threadIdx.x & 31;
-    const int64_t t = w / segs, seg = w - t * segs;
-    if (t >= n_tokens) return;
-    float acc[P::N] = {};
-    const bool mine = P::col(seg, lane, 0) < H;
-    for (int j0 = 0; j0 < k; j0 += 32) {
-        const bool has = j0 + lane < k;
-        int32_t pl = has ? __ldg(place + t * k + j0 + lane) : -1;
-        if (pl >= R) pl = -1;
-        const float pr = has && probs ? load_as_float(probs, probs_type, t * k + j0 + lane) : 1.f;
-        const int n = k - j0 < 32 ? k - j0 : 32;
-        for (int j1 = 0; j1 < n; j1 += GATHER_J) {
-            if constexpr (VEC) {
-                uint4 v[GATHER_J];
+    const int64_t w0 = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), warps = (int64_t)gridDim.x * 8;
+    const int64_t t_step = warps / segs;
+    const int seg_step = (int)(warps - t_step * segs);
+    int64_t t = w0 / segs;
+    int seg = (int)(w0 - t * segs);
+    int32_t next_pl = -1;
+    float next_pr = 0.f;
+    auto fetch = [&](int64_t tt, int j0) {                // a pair without a row has weight 0 and is not loaded
+        int32_t pl = -1;
+        float pr = 0.f;
+        if (tt < n_tokens && j0 + lane < k) {
+            pl = __ldg(place + tt * k + j0 + lane);
+            pr = probs ? load_as_float(probs, probs_type, tt * k + j0 + lane) : 1.f;
+        }
+        next_pl = pl < R ? pl : -1;
+        next_pr = next_pl >= 0 ? pr : 0.f;
+    };
+    fetch(t, 0);
+    while (t < n_tokens) {
+        int64_t t2 = t + t_step;
+        int seg2 = seg + seg_step;
+        if (seg2 >= segs) { seg2 -= segs; ++t2; }
+        const uint32_t off = (uint32_t)(seg * 32 + lane) * B;
+        const bool mine = off < pitch;
+        uint64_t acc[PAIRS];
 #pragma unroll
-                for (int j = 0; j < GATHER_J; ++j) {
-                    const int32_t r = __shfl_sync(0xffffffffu, pl, (j1 + j) & 31);
-                    if (j1 + j < n && r >= 0 && mine) v[j] = P::fetch(rows, r, H, seg, lane);
+        for (int i = 0; i < PAIRS; ++i) acc[i] = 0ull;
+        for (int j0 = 0; j0 < k; j0 += 32) {
+            const int32_t pl = next_pl;
+            const float pr = next_pr;
+            if (j0 + 32 < k) fetch(t, j0 + 32);
+            else fetch(t2, 0);
+            const int n = k - j0 < 32 ? k - j0 : 32;
+            for (int j1 = 0; j1 < n; j1 += J) {
+                uint32_t v[J][W];
+#pragma unroll
+                for (int j = 0; j < J; ++j) {
+                    const int32_t r = __shfl_sync(0xffffffffu, pl, j1 + j);
+#pragma unroll
+                    for (int i = 0; i < W; ++i) v[j][i] = 0u;
+                    if (r >= 0 && mine) load_bytes<B>(rows + off + (uint64_t)(uint32_t)r * pitch, v[j]);
                 }
 #pragma unroll
-                for (int j = 0; j < GATHER_J; ++j) {
-                    const int32_t r = __shfl_sync(0xffffffffu, pl, (j1 + j) & 31);
-                    const float f = __shfl_sync(0xffffffffu, pr, (j1 + j) & 31);
-                    if (j1 + j < n && r >= 0 && mine) {
-                        float x[P::N];
-                        P::widen(v[j], x);
+                for (int j = 0; j < J; ++j) {
+                    const uint32_t f = __float_as_uint(__shfl_sync(0xffffffffu, pr, j1 + j));
+                    const uint64_t f2 = pack2(f, f);
 #pragma unroll
-                        for (int i = 0; i < P::N; ++i) acc[i] += f * x[i];
+                    for (int i = 0; i < PAIRS; ++i) {
+                        uint64_t x;
+                        if constexpr (T == ET_F32) x = pack2(v[j][2 * i], v[j][2 * i + 1]);
+                        else if constexpr (T == ET_BF16) x = pack2(v[j][i] << 16, v[j][i] & 0xFFFF0000u);
+                        else {
+                            const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&v[j][i]));
+                            x = pack2(__float_as_uint(h.x), __float_as_uint(h.y));
+                        }
+                        fma2(acc[i], x, f2);
                     }
-                }
-            } else {
-                for (int j = j1; j < n && j < j1 + GATHER_J; ++j) {
-                    const int32_t r = __shfl_sync(0xffffffffu, pl, j);
-                    const float f = __shfl_sync(0xffffffffu, pr, j);
-                    if (r < 0) continue;
-                    float x[P::N];
-                    P::load(rows, r, H, seg, lane, x);
-#pragma unroll
-                    for (int i = 0; i < P::N; ++i) acc[i] += f * x[i];
                 }
             }
         }
+        if (mine) {
+            uint32_t o[W];
+#pragma unroll
+            for (int i = 0; i < PAIRS; ++i) {
+                float a, b;
+                unpack2(acc[i], a, b);
+                if constexpr (T == ET_F32) { o[2 * i] = __float_as_uint(a); o[2 * i + 1] = __float_as_uint(b); }
+                else if constexpr (T == ET_BF16) { __nv_bfloat162 h = __floats2bfloat162_rn(a, b); o[i] = *reinterpret_cast<uint32_t *>(&h); }
+                else { __half2 h = __floats2half2_rn(a, b); o[i] = *reinterpret_cast<uint32_t *>(&h); }
+            }
+            uint4 *dst = reinterpret_cast<uint4 *>(out + (uint64_t)t * pitch + off);
+#pragma unroll
+            for (int i = 0; i < W / 4; ++i) dst[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        }
+        t = t2;
+        seg = seg2;
     }
-    P::store(out, t, H, seg, lane, acc);
+}
+// Rows whose pieces are not 16-byte aligned: a warp per token and 32 columns at a time.
+template <int T>
+__global__ void __launch_bounds__(256) moe_gather_scalar_kernel(const void *rows, const int32_t *place, const void *probs, int probs_type, void *out,
+                                                                int64_t n_tokens, int k, int64_t R, int64_t H, int segs) {
+    using P = RowPiece<T, false>;
+    const int lane = threadIdx.x & 31;
+    const int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), warps = (int64_t)gridDim.x * 8;
+    for (int64_t item = w; item < n_tokens * segs; item += warps) {
+        const int64_t t = item / segs, seg = item - t * segs;
+        float acc[P::N] = {};
+        for (int j = 0; j < k; ++j) {
+            const int32_t r = __ldg(place + t * k + j);
+            if (r < 0 || r >= R) continue;
+            const float f = probs ? load_as_float(probs, probs_type, t * k + j) : 1.f;
+            float x[P::N];
+            P::load(rows, r, H, seg, lane, x);
+#pragma unroll
+            for (int i = 0; i < P::N; ++i) acc[i] = fmaf(f, x[i], acc[i]);
+        }
+        P::store(out, t, H, seg, lane, acc);
+    }
 }
 
 // ---- gradients of the weighted sum ---------------------------------------------------------------
-// A CTA per token: its warps share the row's segments, write probs * gradOut into each of the token's rows and sum
-// <gradOut, row>; the warps' sums meet in shared memory in a fixed order.
-constexpr int GRAD_J = 8;
-template <int T, bool VEC>
+// A CTA per token in turn: its warps share the row's pieces, write probs * gradOut into each of the token's rows and sum
+// <gradOut, row>; the warps' sums meet in shared memory in a fixed order.  J pairs at a time.
+template <int T, bool VEC, int J>
 __global__ void __launch_bounds__(256) moe_gather_grad_kernel(const void *dout, const void *rows, const int32_t *place, const void *probs, int probs_type,
-                                                              void *drows, void *dprobs, int k, int64_t R, int64_t H, int64_t segs) {
+                                                              void *drows, void *dprobs, int64_t n_tokens, int k, int64_t R, int64_t H, int segs) {
     using P = RowPiece<T, VEC>;
-    __shared__ float part[8][GRAD_J];
-    const int64_t t = blockIdx.x;
+    __shared__ float part[2][8][J];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    for (int j0 = 0; j0 < k; j0 += GRAD_J) {
-        float dot[GRAD_J], pr[GRAD_J];
-        int32_t pl[GRAD_J];
-#pragma unroll
-        for (int j = 0; j < GRAD_J; ++j) {
-            dot[j] = 0.f;
-            const bool has = j0 + j < k;
-            pl[j] = has ? __ldg(place + t * k + j0 + j) : -1;
-            if (pl[j] >= R) pl[j] = -1;
-            pr[j] = has ? load_as_float(probs, probs_type, t * k + j0 + j) : 0.f;
+    int32_t next_pl = -1;
+    float next_pr = 0.f;
+    auto fetch = [&](int64_t tt, int j0) {
+        next_pl = -1;
+        if (tt < n_tokens && lane < J && j0 + lane < k) {
+            next_pl = __ldg(place + tt * k + j0 + lane);
+            next_pr = load_as_float(probs, probs_type, tt * k + j0 + lane);
         }
-        for (int64_t seg = warp; seg < segs; seg += warps) {
-            float g[P::N];
-            uint4 raw[GRAD_J];
-            if constexpr (VEC) {
-                if (P::col(seg, lane, 0) < H) {
+    };
+    fetch(blockIdx.x, 0);
+    int buf = 0;
+    for (int64_t t = blockIdx.x; t < n_tokens; t += gridDim.x) {
+        for (int j0 = 0; j0 < k; j0 += J) {
+            float dot[J], pr[J];
+            int32_t pl[J];
 #pragma unroll
-                    for (int j = 0; j < GRAD_J; ++j)
-                        if (pl[j] >= 0) raw[j] = P::fetch(rows, pl[j], H, seg, lane);
-                }
+            for (int j = 0; j < J; ++j) {
+                dot[j] = 0.f;
+                pl[j] = __shfl_sync(0xffffffffu, next_pl < R ? next_pl : -1, j);
+                pr[j] = __shfl_sync(0xffffffffu, next_pr, j);
             }
-            P::load(dout, t, H, seg, lane, g);
-#pragma unroll
-            for (int j = 0; j < GRAD_J; ++j) {
-                if (pl[j] < 0) continue;
-                float v[P::N], o[P::N];
+            if (j0 + J < k) fetch(t, j0 + J);
+            else fetch(t + gridDim.x, 0);
+            for (int seg = warp; seg < segs; seg += warps) {
+                float g[P::N];
+                uint4 raw[J];
                 if constexpr (VEC) {
-                    if (P::col(seg, lane, 0) >= H) continue;
-                    P::widen(raw[j], v);
-                } else {
-                    P::load(rows, pl[j], H, seg, lane, v);
+                    if (P::col(seg, lane, 0) < H) {
+#pragma unroll
+                        for (int j = 0; j < J; ++j)
+                            if (pl[j] >= 0) raw[j] = P::fetch(rows, pl[j], H, seg, lane);
+                    }
                 }
+                P::load(dout, t, H, seg, lane, g);
 #pragma unroll
-                for (int i = 0; i < P::N; ++i) { dot[j] += g[i] * v[i]; o[i] = pr[j] * g[i]; }
-                P::store(drows, pl[j], H, seg, lane, o);
+                for (int j = 0; j < J; ++j) {
+                    if (pl[j] < 0) continue;
+                    float v[P::N], o[P::N];
+                    if constexpr (VEC) {
+                        if (P::col(seg, lane, 0) >= H) continue;
+                        P::widen(raw[j], v);
+                    } else {
+                        P::load(rows, pl[j], H, seg, lane, v);
+                    }
+#pragma unroll
+                    for (int i = 0; i < P::N; ++i) { dot[j] += g[i] * v[i]; o[i] = pr[j] * g[i]; }
+                    P::store(drows, pl[j], H, seg, lane, o);
+                }
             }
-        }
 #pragma unroll
-        for (int j = 0; j < GRAD_J; ++j) {
+            for (int j = 0; j < J; ++j) {
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], o);
-            if (lane == 0) part[warp][j] = dot[j];
+                for (int o = 16; o > 0; o >>= 1) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], o);
+                if (lane == 0) part[buf][warp][j] = dot[j];
+            }
+            __syncthreads();
+            if (threadIdx.x < J && j0 + threadIdx.x < k) {
+                float s = 0.f;
+                for (int w = 0; w < warps; ++w) s += part[buf][w][threadIdx.x];
+                store_from_float(dprobs, probs_type, t * k + j0 + threadIdx.x, s);
+            }
+            buf ^= 1;   // the next round's sums go to the other half: one barrier a round is enough
         }
-        __syncthreads();
-        if (threadIdx.x < GRAD_J && j0 + threadIdx.x < k) {
-            float s = 0.f;
-            for (int w = 0; w < warps; ++w) s += part[w][threadIdx.x];
-            store_from_float(dprobs, probs_type, t * k + j0 + threadIdx.x, s);
-        }
-        __syncthreads();
     }
 }
 
@@ -369,17 +465,18 @@ template <typename U> cudaError_t launch_permute(const PermuteArgs &p, cudaStrea
         count_launch();
         return cudaGetLastError();
     }
-    cudaError_t e = allow_smem<moe_sort_kernel>((SORT_WARPS + 1) * MOE_MAX_EXPERTS * 4);
+    cudaError_t e = allow_smem<moe_sort_kernel>((SORT_WARPS + 2) * MOE_MAX_EXPERTS * 4);
     if (e != cudaSuccess) return e;
-    moe_sort_kernel<<<SORT_CTAS, SORT_WARPS * 32, (size_t)(SORT_WARPS + 1) * p.E * 4, s>>>(p.ids, p.ids64, p.place, p.counts, N, (int)p.E);
+    moe_sort_kernel<<<SORT_CTAS, SORT_WARPS * 32, (size_t)(SORT_WARPS + 2) * p.E * 4, s>>>(p.ids, p.ids64, p.place, p.counts, N, (int)p.E);
     count_launch();
     e = cudaGetLastError();
     if (e != cudaSuccess || (units == 0 && p.S == 0)) return e;
     const int64_t segs = units > 128 ? (units + 127) / 128 : 1, ctas = (p.T * segs + 7) / 8;
     if (ctas > 0x7fffffffLL) return cudaErrorInvalidValue;
-    moe_scatter_kernel<U><<<(unsigned)ctas, 256, 0, s>>>((const U *)p.tokens, p.scales, p.place, (U *)p.rows, p.scales_out, p.T, (int)p.k, units, p.S, segs);
-    count_launch();
-    return cudaGetLastError();
+    e = launch_chained(moe_scatter_kernel<U>, (unsigned)ctas, 256, 0, 1, s, (const U *)p.tokens, p.scales, (const int32_t *)p.place, (U *)p.rows, p.scales_out,
+                       p.T, (int)p.k, units, p.S, segs);
+    if (e == cudaSuccess) count_launch();
+    return e;
 }
 
 }  // namespace
@@ -395,18 +492,21 @@ cudaError_t launch_moe_permute(const PermuteArgs &p, cudaStream_t s) {
 cudaError_t launch_moe_unpermute(const void *rows, int type, const int32_t *place, const void *probs, int probs_type, void *out,
                                  int64_t T, int64_t k, int64_t R, int64_t H, cudaStream_t s) {
     if (T <= 0 || H <= 0) return cudaSuccess;
+    const int64_t pitch = H * (type == ET_F32 ? 4 : 2);
+    const uint64_t all = reinterpret_cast<uintptr_t>(rows) | reinterpret_cast<uintptr_t>(out) | (uint64_t)pitch;
+    // 32 bytes a lane where the rows allow it and are long enough to fill the warp with them
+    const int bytes = all % 32 == 0 && pitch >= 1024 ? 32 : 16;
     const int per = type == ET_F32 ? 4 : 8;
-    const bool vec = H % per == 0 && aligned16(rows) && aligned16(out);
-    const int64_t segs = (H + 32 * per - 1) / (32 * per), ctas = (T * segs + 7) / 8;
-    if (ctas > 0x7fffffffLL) return cudaErrorInvalidValue;
-#define MG(TT) do { if (vec) moe_gather_kernel<TT, true><<<(unsigned)ctas, 256, 0, s>>>(rows, place, probs, probs_type, out, T, (int)k, R, H, segs); \
-                    else moe_gather_kernel<TT, false><<<(unsigned)ctas, 256, 0, s>>>(rows, place, probs, probs_type, out, T, (int)k, R, H, segs); } while (0)
-    if (type == ET_BF16) MG(ET_BF16);
-    else if (type == ET_F16) MG(ET_F16);
-    else MG(ET_F32);
+    const bool vec = all % 16 == 0 && pitch < (1LL << 31);
+    const int64_t segs = vec ? (pitch + 32 * bytes - 1) / (32 * bytes) : (H + 32 * per - 1) / (32 * per);
+    if (segs > 0x7fffffffLL) return cudaErrorInvalidValue;
+    const int64_t ctas = (T * segs + 7) / 8;
+#define MGB(TT, B, J) launch_resident<moe_gather_kernel<TT, B, J>>(ctas, 256, s, (const char *)rows, place, probs, probs_type, (char *)out, T, (int)k, R, (uint32_t)pitch, (int)segs)
+#define MG(TT) (!vec ? launch_resident<moe_gather_scalar_kernel<TT>>(ctas, 256, s, rows, place, probs, probs_type, out, T, (int)k, R, H, (int)segs) \
+                     : (bytes == 32 ? MGB(TT, 32, 4) : (k <= 4 ? MGB(TT, 16, 4) : MGB(TT, 16, 8))))
+    return type == ET_BF16 ? MG(ET_BF16) : (type == ET_F16 ? MG(ET_F16) : MG(ET_F32));
 #undef MG
-    count_launch();
-    return cudaGetLastError();
+#undef MGB
 }
 
 cudaError_t launch_moe_unpermute_grad(const void *dout, const void *rows, int type, const int32_t *place, const void *probs, int probs_type,
@@ -415,15 +515,13 @@ cudaError_t launch_moe_unpermute_grad(const void *dout, const void *rows, int ty
     const int per = type == ET_F32 ? 4 : 8;
     const bool vec = H % per == 0 && aligned16(dout) && aligned16(rows) && aligned16(drows);
     const int64_t segs = (H + 32 * per - 1) / (32 * per);
-    const unsigned threads = (unsigned)(segs < 1 ? 32 : (segs < 8 ? 32 * segs : 256));
-#define MGG(TT) do { if (vec) moe_gather_grad_kernel<TT, true><<<(unsigned)T, threads, 0, s>>>(dout, rows, place, probs, probs_type, drows, dprobs, (int)k, R, H, segs); \
-                     else moe_gather_grad_kernel<TT, false><<<(unsigned)T, threads, 0, s>>>(dout, rows, place, probs, probs_type, drows, dprobs, (int)k, R, H, segs); } while (0)
-    if (type == ET_BF16) MGG(ET_BF16);
-    else if (type == ET_F16) MGG(ET_F16);
-    else MGG(ET_F32);
+    if (segs > 0x7fffffffLL) return cudaErrorInvalidValue;
+    const int threads = segs < 1 ? 32 : (segs < 8 ? 32 * (int)segs : 256);
+#define MGJ(TT, V, J) launch_resident<moe_gather_grad_kernel<TT, V, J>>(T, threads, s, dout, rows, place, probs, probs_type, drows, dprobs, T, (int)k, R, H, (int)segs)
+#define MGG(TT) (vec ? (k <= 4 ? MGJ(TT, true, 4) : MGJ(TT, true, 8)) : MGJ(TT, false, 8))
+    return type == ET_BF16 ? MGG(ET_BF16) : (type == ET_F16 ? MGG(ET_F16) : MGG(ET_F32));
 #undef MGG
-    count_launch();
-    return cudaGetLastError();
+#undef MGJ
 }
 
 }  // namespace qmm

@@ -9,8 +9,10 @@
 // SwiGLU uses the fast exponential and quotient (a few 2^-23 of the value, against a code's 2^-4): with expf and an IEEE division
 // per element the kernel was bound by instruction issue (4099 x 14336 bf16: 83 us).
 //
-// HBM-bound: each value is read once and each code written once.  A half-warp owns a block: 8 values per lane (one
-// 16-byte load of a 16-bit type, two of fp32), the maximum by four shuffles, 8 codes per lane in one 8-byte store.
+// HBM-bound: each value is read once and each code written once, so the rest has to stay below some 16 instructions a
+// value.  A lane owns 16 values of a 16-bit type (one 32-byte load, one 16-byte store), 8 of fp32, so that 8 or 16 lanes own a
+// block and share its maximum by three or four shuffles; with 8 values a lane the two divisions per block and the
+// addresses were done twice as often (4099 x 14336 bf16: 39.7 us).
 #include "device_utils.cuh"
 
 namespace qmm {
@@ -24,74 +26,87 @@ template <bool E5M2> __device__ __forceinline__ float block_scale(float amax) {
     return amax > 0.f ? fmaxf(__fdiv_rn(amax, top), 1.17549435e-38f) : 1.f;
 }
 
-// 8 consecutive elements from x[idx]; with VEC they lie inside the row and the address is 16-byte aligned, else `n` of them do.
-template <int T, bool VEC> __device__ __forceinline__ void load8(const void *x, int64_t idx, int n, float (&f)[8]) {
-    if constexpr (VEC) {
-        if (n <= 0) {
+// N consecutive elements as fp32 from x[idx] (N * size is 16 or 32 bytes, aligned), or `n` of them one by one.
+template <int T, int N> struct Lane {
+    static constexpr int W = N * (T == ET_F32 ? 4 : 2) / 4;
+    uint32_t w[W];
+    __device__ __forceinline__ void load(const void *x, int64_t idx, bool in) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = 0.f;
-            return;
+        for (int i = 0; i < W; ++i) w[i] = 0u;
+        if (!in) return;
+        const char *p = (const char *)x + idx * (T == ET_F32 ? 4 : 2);
+        if constexpr (W == 8)
+            asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7]) : "l"(p));
+        else {
+            const uint4 v = __ldg(reinterpret_cast<const uint4 *>(p));
+            w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
         }
-        if constexpr (T == ET_F32) {
-            const float4 a = __ldg(reinterpret_cast<const float4 *>((const float *)x + idx));
-            const float4 b = __ldg(reinterpret_cast<const float4 *>((const float *)x + idx) + 1);
-            f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-        } else {
-            const uint4 v = __ldg(reinterpret_cast<const uint4 *>((const uint16_t *)x + idx));
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    }
+    __device__ __forceinline__ void widen(float (&f)[N]) const {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if constexpr (T == ET_BF16) { f[2 * i] = __uint_as_float(w[i] << 16); f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u); }
-                else { f[2 * i] = __half2float(__ushort_as_half((unsigned short)(w[i] & 0xFFFFu))); f[2 * i + 1] = __half2float(__ushort_as_half((unsigned short)(w[i] >> 16))); }
-            }
+        for (int i = 0; i < W; ++i) {
+            if constexpr (T == ET_F32) f[i] = __uint_as_float(w[i]);
+            else if constexpr (T == ET_BF16) { f[2 * i] = __uint_as_float(w[i] << 16); f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u); }
+            else { const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&w[i])); f[2 * i] = h.x; f[2 * i + 1] = h.y; }
+        }
+    }
+};
+template <int T, int N> __device__ __forceinline__ void load_each(const void *x, int64_t idx, int n, float (&f)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = i < n ? load_as_float(x, T, idx + i) : 0.f;
+}
+
+// Rows of D; block b covers columns 128 c .. of row r with b = r * kb + c.  N values a lane, VEC: D is a multiple of N and the
+// addresses are aligned, so that a lane's values are inside the row or none is.
+template <int T, int N, bool VEC, bool SWIGLU, bool E5M2>
+__global__ void __launch_bounds__(256) block_quant_kernel(const void *x, uint8_t *q, float *scale_out, uint32_t nblocks, uint32_t kb, int64_t D) {
+    constexpr int LPB = 128 / N;                          // lanes of a block
+    const uint32_t b = blockIdx.x * (256u / LPB) + threadIdx.x / LPB, r = b / kb;
+    const int c0 = (threadIdx.x % LPB) * N;
+    const int64_t col = (int64_t)(b - r * kb) * 128 + c0, rest = D - col, at = (int64_t)r * D + col;
+    const int left = b < nblocks ? (int)(rest > N ? N : rest) : 0;
+    const int64_t in = SWIGLU ? at + (int64_t)r * D : at;
+    float f[N], m = 0.f;
+    if constexpr (VEC) {
+        Lane<T, N> a, g;
+        a.load(x, in, left > 0);
+        if constexpr (SWIGLU) g.load(x, in + D, left > 0);
+        a.widen(f);
+        if constexpr (SWIGLU) {
+            float h[N];
+            g.widen(h);
+#pragma unroll
+            for (int i = 0; i < N; ++i) f[i] = __fdividef(f[i], 1.f + __expf(-f[i])) * h[i];
+        }
+    } else {
+        load_each<T, N>(x, in, left, f);
+        if constexpr (SWIGLU) {
+            float h[N];
+            load_each<T, N>(x, in + D, left, h);
+#pragma unroll
+            for (int i = 0; i < N; ++i) f[i] = __fdividef(f[i], 1.f + __expf(-f[i])) * h[i];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) m = fmaxf(m, fabsf(f[i]));
+#pragma unroll
+    for (int o = LPB / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float sc = block_scale<E5M2>(m), inv = __frcp_rn(sc);
+    if (c0 == 0 && b < nblocks) scale_out[b] = sc;
+    uint32_t w[N / 4];
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i)
+        w[i] = codes2<E5M2>(f[4 * i] * inv, f[4 * i + 1] * inv) | (codes2<E5M2>(f[4 * i + 2] * inv, f[4 * i + 3] * inv) << 16);
+    if constexpr (VEC) {
+        if (left > 0) {
+            if constexpr (N == 16) *reinterpret_cast<uint4 *>(q + at) = make_uint4(w[0], w[1], w[2], w[3]);
+            else *reinterpret_cast<uint2 *>(q + at) = make_uint2(w[0], w[1]);
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = i < n ? load_as_float(x, T, idx + i) : 0.f;
-    }
-}
-
-// Rows of D; block b covers columns 128 c .. of row r with b = r * kb + c.  UNROLL blocks per half-warp are in flight.
-template <int T, bool VEC, bool SWIGLU, bool E5M2, int UNROLL>
-__global__ void __launch_bounds__(256) block_quant_kernel(const void *x, uint8_t *q, float *scale_out, uint32_t nblocks, uint32_t kb, int64_t D) {
-    const uint32_t b0 = blockIdx.x * (16u * UNROLL) + (threadIdx.x >> 4);
-    const int c8 = (threadIdx.x & 15) * 8;
-    float f[UNROLL][8], g[SWIGLU ? UNROLL : 1][8];
-    int64_t at[UNROLL];
-    int left[UNROLL];
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-        const uint32_t b = b0 + 16u * u, r = b / kb;
-        const int64_t col = (int64_t)(b - r * kb) * 128 + c8, rest = D - col;
-        left[u] = b < nblocks ? (int)(rest > 8 ? 8 : rest) : 0;
-        at[u] = (int64_t)r * D + col;
-        const int64_t in = SWIGLU ? at[u] + (int64_t)r * D : at[u];
-        load8<T, VEC>(x, in, left[u], f[u]);
-        if constexpr (SWIGLU) load8<T, VEC>(x, in + D, left[u], g[u]);
-    }
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-        float m = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if constexpr (SWIGLU) f[u][i] = __fdividef(f[u][i], 1.f + __expf(-f[u][i])) * g[u][i];
-            m = fmaxf(m, fabsf(f[u][i]));
-        }
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        const float sc = block_scale<E5M2>(m), inv = __frcp_rn(sc);
-        const uint32_t b = b0 + 16u * u;
-        if (c8 == 0 && b < nblocks) scale_out[b] = sc;
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = codes2<E5M2>(f[u][2 * i] * inv, f[u][2 * i + 1] * inv);
-        if constexpr (VEC) {
-            if (left[u] > 0) *reinterpret_cast<uint2 *>(q + at[u]) = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (i < left[u]) q[at[u] + i] = (uint8_t)(w[i >> 1] >> (8 * (i & 1)));
-        }
+        for (int i = 0; i < N; ++i)
+            if (i < left) q[at + i] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
     }
 }
 
@@ -106,7 +121,14 @@ __global__ void __launch_bounds__(256) tile_quant_kernel(const void *x, uint8_t 
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const int64_t r = r0 + (threadIdx.x >> 4) + 16 * i;
-        load8<T, VEC>(x, r * D + col, r < rows ? (int)(rest > 8 ? 8 : rest) : 0, f[i]);
+        const int left = r < rows ? (int)(rest > 8 ? 8 : rest) : 0;
+        if constexpr (VEC && T != ET_F32) {
+            Lane<T, 8> a;
+            a.load(x, r * D + col, left > 0);
+            a.widen(f[i]);
+        } else {
+            load_each<T, 8>(x, r * D + col, left, f[i]);
+        }
 #pragma unroll
         for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(f[i][j]));
     }
@@ -131,21 +153,35 @@ __global__ void __launch_bounds__(256) tile_quant_kernel(const void *x, uint8_t 
     }
 }
 
-template <int T, bool VEC, bool E5M2>
-cudaError_t launch_typed(const void *x, int64_t row_block, bool swiglu, uint8_t *q, float *scale_out, int64_t rows, int64_t D, cudaStream_t s) {
-    const uint32_t kb = (uint32_t)((D + 127) / 128);
-    if (row_block == 128) {
-        const int64_t n = (rows + 127) / 128 * kb;
-        if (n > 0x7fffffffLL) return cudaErrorInvalidValue;
-        tile_quant_kernel<T, VEC, E5M2><<<(unsigned)n, 256, 0, s>>>(x, q, scale_out, rows, kb, D);
-    } else {
-        const int64_t n = rows * kb;
-        if (n > 0x7fffffffLL) return cudaErrorInvalidValue;
-        if (swiglu) block_quant_kernel<T, VEC, true, E5M2, 1><<<(unsigned)((n + 15) / 16), 256, 0, s>>>(x, q, scale_out, (uint32_t)n, kb, D);
-        else block_quant_kernel<T, VEC, false, E5M2, 1><<<(unsigned)((n + 15) / 16), 256, 0, s>>>(x, q, scale_out, (uint32_t)n, kb, D);
-    }
+template <int T, int N, bool VEC, bool E5M2>
+cudaError_t launch_rows(const void *x, bool swiglu, uint8_t *q, float *scale_out, int64_t rows, int64_t D, cudaStream_t s) {
+    const int64_t kb = (D + 127) / 128, n = rows * kb;
+    if (n > 0x7fffffffLL) return cudaErrorInvalidValue;
+    constexpr int PER_CTA = 256 / (128 / N);
+    const unsigned g = (unsigned)((n + PER_CTA - 1) / PER_CTA);
+    if (swiglu) block_quant_kernel<T, N, VEC, true, E5M2><<<g, 256, 0, s>>>(x, q, scale_out, (uint32_t)n, (uint32_t)kb, D);
+    else block_quant_kernel<T, N, VEC, false, E5M2><<<g, 256, 0, s>>>(x, q, scale_out, (uint32_t)n, (uint32_t)kb, D);
     count_launch();
     return cudaGetLastError();
+}
+template <int T, bool E5M2>
+cudaError_t launch_typed(const void *x, int64_t row_block, bool swiglu, uint8_t *q, float *scale_out, int64_t rows, int64_t D, cudaStream_t s) {
+    const uint64_t ax = reinterpret_cast<uintptr_t>(x), aq = reinterpret_cast<uintptr_t>(q);
+    if (row_block == 128) {
+        const int64_t kb = (D + 127) / 128, n = (rows + 127) / 128 * kb;
+        if (n > 0x7fffffffLL) return cudaErrorInvalidValue;
+        if (D % 8 == 0 && ax % 16 == 0) tile_quant_kernel<T, true, E5M2><<<(unsigned)n, 256, 0, s>>>(x, q, scale_out, rows, (uint32_t)kb, D);
+        else tile_quant_kernel<T, false, E5M2><<<(unsigned)n, 256, 0, s>>>(x, q, scale_out, rows, (uint32_t)kb, D);
+        count_launch();
+        return cudaGetLastError();
+    }
+    if constexpr (T == ET_F32) {
+        if (D % 8 == 0 && ax % 32 == 0 && aq % 8 == 0) return launch_rows<T, 8, true, E5M2>(x, swiglu, q, scale_out, rows, D, s);
+    } else {
+        if (D % 16 == 0 && ax % 32 == 0 && aq % 16 == 0) return launch_rows<T, 16, true, E5M2>(x, swiglu, q, scale_out, rows, D, s);
+        if (D % 8 == 0 && ax % 16 == 0 && aq % 8 == 0) return launch_rows<T, 8, true, E5M2>(x, swiglu, q, scale_out, rows, D, s);
+    }
+    return launch_rows<T, 8, false, E5M2>(x, swiglu, q, scale_out, rows, D, s);
 }
 
 }  // namespace
@@ -153,12 +189,8 @@ cudaError_t launch_typed(const void *x, int64_t row_block, bool swiglu, uint8_t 
 cudaError_t launch_block_quant(const void *x, int x_type, int64_t row_block, bool swiglu, uint8_t *q, int q_type, float *scale_out,
                                int64_t rows, int64_t D, cudaStream_t s) {
     if (rows <= 0 || D <= 0) return cudaSuccess;
-    const bool vec = D % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (reinterpret_cast<uintptr_t>(q) & 7) == 0;
     const bool e5 = q_type == ET_E5M2;
-#define BQ(T) (vec ? (e5 ? launch_typed<T, true, true>(x, row_block, swiglu, q, scale_out, rows, D, s)    \
-                         : launch_typed<T, true, false>(x, row_block, swiglu, q, scale_out, rows, D, s))  \
-                   : (e5 ? launch_typed<T, false, true>(x, row_block, swiglu, q, scale_out, rows, D, s)   \
-                         : launch_typed<T, false, false>(x, row_block, swiglu, q, scale_out, rows, D, s)))
+#define BQ(T) (e5 ? launch_typed<T, true>(x, row_block, swiglu, q, scale_out, rows, D, s) : launch_typed<T, false>(x, row_block, swiglu, q, scale_out, rows, D, s))
     if (x_type == ET_BF16) return BQ(ET_BF16);
     if (x_type == ET_F16) return BQ(ET_F16);
     return BQ(ET_F32);

@@ -52,20 +52,22 @@ template <int T, int N> struct Lane {
         }
     }
 };
-template <int T, int N> __device__ __forceinline__ void load_each(const void *x, int64_t idx, int n, float (&f)[N]) {
+// N elements STEP apart, as far as they lie in front of `n`.
+template <int T, int N, int STEP> __device__ __forceinline__ void load_each(const void *x, int64_t idx, int64_t n, float (&f)[N]) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) f[i] = i < n ? load_as_float(x, T, idx + i) : 0.f;
+    for (int i = 0; i < N; ++i) f[i] = i * STEP < n ? load_as_float(x, T, idx + i * STEP) : 0.f;
 }
 
 // Rows of D; block b covers columns 128 c .. of row r with b = r * kb + c.  N values a lane, VEC: D is a multiple of N and the
-// addresses are aligned, so that a lane's values are inside the row or none is.
+// addresses are aligned, so that a lane's values, next to each other, are inside the row or none is.  Else they are as far
+// apart as the block has lanes, so that the lanes' single accesses lie side by side.
 template <int T, int N, bool VEC, bool SWIGLU, bool E5M2>
 __global__ void __launch_bounds__(256) block_quant_kernel(const void *x, uint8_t *q, float *scale_out, uint32_t nblocks, uint32_t kb, int64_t D) {
     constexpr int LPB = 128 / N;                          // lanes of a block
     const uint32_t b = blockIdx.x * (256u / LPB) + threadIdx.x / LPB, r = b / kb;
-    const int c0 = (threadIdx.x % LPB) * N;
+    const int c0 = (threadIdx.x % LPB) * (VEC ? N : 1);
     const int64_t col = (int64_t)(b - r * kb) * 128 + c0, rest = D - col, at = (int64_t)r * D + col;
-    const int left = b < nblocks ? (int)(rest > N ? N : rest) : 0;
+    const int left = b < nblocks ? (int)(rest > 128 - c0 ? 128 - c0 : rest) : 0;   // of the block and the row, from this lane's first
     const int64_t in = SWIGLU ? at + (int64_t)r * D : at;
     float f[N], m = 0.f;
     if constexpr (VEC) {
@@ -80,10 +82,10 @@ __global__ void __launch_bounds__(256) block_quant_kernel(const void *x, uint8_t
             for (int i = 0; i < N; ++i) f[i] = __fdividef(f[i], 1.f + __expf(-f[i])) * h[i];
         }
     } else {
-        load_each<T, N>(x, in, left, f);
+        load_each<T, N, LPB>(x, in, left, f);
         if constexpr (SWIGLU) {
             float h[N];
-            load_each<T, N>(x, in + D, left, h);
+            load_each<T, N, LPB>(x, in + D, left, h);
 #pragma unroll
             for (int i = 0; i < N; ++i) f[i] = __fdividef(f[i], 1.f + __expf(-f[i])) * h[i];
         }
@@ -106,7 +108,7 @@ __global__ void __launch_bounds__(256) block_quant_kernel(const void *x, uint8_t
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i)
-            if (i < left) q[at + i] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
+            if (i * LPB < left) q[at + i * LPB] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
     }
 }
 
@@ -127,7 +129,7 @@ __global__ void __launch_bounds__(256) tile_quant_kernel(const void *x, uint8_t 
             a.load(x, r * D + col, left > 0);
             a.widen(f[i]);
         } else {
-            load_each<T, 8>(x, r * D + col, left, f[i]);
+            load_each<T, 8, 1>(x, r * D + col, left, f[i]);
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(f[i][j]));

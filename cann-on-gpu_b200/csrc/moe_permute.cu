@@ -20,7 +20,7 @@ __device__ __forceinline__ int expert_of(const void *ids, bool ids64, int64_t i,
 
 // ---- the sort: one cluster of 8 CTAs, no workspace ------------------------------------------------
 // The pairs are cut into 8 x 32 contiguous warp shares.  Pass 1 counts experts per warp (lanes of one expert find each
-// other with match_any), then each expert's counts are summed over the warps before, the CTAs before (distributed shared
+// other by a ballot per bit of the expert's number: 4 instructions each, where match_any took about 270 cycles), then each expert's counts are summed over the warps before, the CTAs before (distributed shared
 // memory) and the experts before; pass 2 walks the shares again and hands out places in order.
 constexpr int SORT_CTAS = 8, SORT_WARPS = 32;
 
@@ -34,8 +34,20 @@ __device__ __forceinline__ int ld_remote(const int *local, int cta) {
     return v;
 }
 
-// (Eight ids of a lane are loaded at once: one at a time, 65536 pairs took 22 us, two thirds of it load latency.)
+// Eight ids of a lane are loaded at once, and up to 65536 pairs they stay in registers for pass 2.
 constexpr int SORT_RUN = 8;
+template <int BITS> __device__ __forceinline__ unsigned lanes_alike(int v) {
+    unsigned same = 0xffffffffu;
+#pragma unroll
+    for (int b = 0; b < BITS; ++b) {
+        const bool one = (v >> b) & 1;
+        const unsigned m = __ballot_sync(0xffffffffu, one);
+        same &= one ? m : ~m;
+    }
+    return same;
+}
+// BITS: enough for 0 .. E, E standing for no expert.
+template <int BITS>
 __global__ void __cluster_dims__(SORT_CTAS, 1, 1) __launch_bounds__(SORT_WARPS * 32)
 moe_sort_kernel(const void *ids, bool ids64, int32_t *place, int64_t *counts, int64_t N, int E) {
     extern __shared__ int hist[];                 // [SORT_WARPS][E], then [E] totals of the CTA, then [E] first places
@@ -43,27 +55,36 @@ moe_sort_kernel(const void *ids, bool ids64, int32_t *place, int64_t *counts, in
     int *cta_total = hist + SORT_WARPS * E, *start = cta_total + E;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, cta = blockIdx.x;
     int *mine = hist + warp * E;
-    for (int i = lane; i < E; i += 32) mine[i] = 0;
-    __syncwarp();
     const int64_t share = (N + SORT_CTAS * SORT_WARPS * 32 - 1) / (SORT_CTAS * SORT_WARPS * 32) * 32;
     const int64_t lo = (int64_t)(cta * SORT_WARPS + warp) * share, hi = lo + share < N ? lo + share : N;
+    const bool kept = share <= 32 * SORT_RUN;     // one run: pass 2 finds everything in registers
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    int e[SORT_RUN];
+    int e[SORT_RUN], at[SORT_RUN];                // expert, and the place among the warp's of that expert
     auto load = [&](int64_t i0) {
 #pragma unroll
         for (int r = 0; r < SORT_RUN; ++r) {
             const int64_t i = i0 + 32 * r + lane;
             e[r] = i < hi ? expert_of(ids, ids64, i, E) : -1;
+            if (e[r] < 0) e[r] = E;
         }
     };
-    for (int64_t i0 = lo; i0 < hi; i0 += 32 * SORT_RUN) {
-        load(i0);
+    auto count = [&](int64_t i0) {
 #pragma unroll
         for (int r = 0; r < SORT_RUN; ++r) {
-            const unsigned same = __match_any_sync(0xffffffffu, e[r]);
-            if (e[r] >= 0 && (same & ((1u << lane) - 1)) == 0) mine[e[r]] += __popc(same);
+            if (i0 + 32 * r >= hi) break;
+            const unsigned same = lanes_alike<BITS>(e[r]), below = same & ((1u << lane) - 1);
+            if (e[r] < E) at[r] = mine[e[r]] + __popc(below);
+            __syncwarp();
+            if (e[r] < E && below == 0) mine[e[r]] += __popc(same);
             __syncwarp();
         }
+    };
+    load(lo);
+    for (int i = lane; i < E; i += 32) mine[i] = 0;
+    __syncwarp();
+    for (int64_t i0 = lo; i0 < hi; i0 += 32 * SORT_RUN) {
+        if (i0 > lo) load(i0);
+        count(i0);
     }
     __syncthreads();
     if (tid < E) {
@@ -96,25 +117,21 @@ moe_sort_kernel(const void *ids, bool ids64, int32_t *place, int64_t *counts, in
     }
     if (lane == 31) scan[warp] = incl;
     __syncthreads();
-    int base = incl - total + before;
-    for (int w = 0; w < warp; ++w) base += scan[w];
+    const int base = incl - total + before + __reduce_add_sync(0xffffffffu, lane < warp ? scan[lane] : 0);
     if (tid < E) {
         start[tid] = base;
         if (cta == 0) counts[tid] = total;
     }
     __syncthreads();
     for (int64_t i0 = lo; i0 < hi; i0 += 32 * SORT_RUN) {
-        if (share > 32 * SORT_RUN) load(i0);      // a single run is still in registers
+        if (!kept) {                              // (the warp's counters, now its first places, count on)
+            load(i0);
+            count(i0);
+        }
 #pragma unroll
         for (int r = 0; r < SORT_RUN; ++r) {
             const int64_t i = i0 + 32 * r + lane;
-            const unsigned same = __match_any_sync(0xffffffffu, e[r]);
-            const unsigned below = same & ((1u << lane) - 1);
-            const int at = e[r] >= 0 ? start[e[r]] + mine[e[r]] + __popc(below) : -1;
-            __syncwarp();
-            if (e[r] >= 0 && below == 0) mine[e[r]] += __popc(same);
-            __syncwarp();
-            if (i < hi) place[i] = at;
+            if (i < hi) place[i] = e[r] < E ? start[e[r]] + at[r] + (kept ? mine[e[r]] : 0) : -1;
         }
     }
     cluster_wait();
@@ -457,6 +474,13 @@ __global__ void __launch_bounds__(256) moe_gather_grad_kernel(const void *dout, 
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+template <int BITS> cudaError_t launch_sort(const PermuteArgs &p, int64_t N, cudaStream_t s) {
+    const cudaError_t e = allow_smem<moe_sort_kernel<BITS>>((SORT_WARPS + 2) * MOE_MAX_EXPERTS * 4);
+    if (e != cudaSuccess) return e;
+    moe_sort_kernel<BITS><<<SORT_CTAS, SORT_WARPS * 32, (size_t)(SORT_WARPS + 2) * p.E * 4, s>>>(p.ids, p.ids64, p.place, p.counts, N, (int)p.E);
+    count_launch();
+    return cudaGetLastError();
+}
 template <typename U> cudaError_t launch_permute(const PermuteArgs &p, cudaStream_t s) {
     const int64_t units = p.row_bytes / (int64_t)sizeof(U), N = p.T * p.k;
     if (N <= SMALL_PAIRS) {
@@ -465,11 +489,9 @@ template <typename U> cudaError_t launch_permute(const PermuteArgs &p, cudaStrea
         count_launch();
         return cudaGetLastError();
     }
-    cudaError_t e = allow_smem<moe_sort_kernel>((SORT_WARPS + 2) * MOE_MAX_EXPERTS * 4);
-    if (e != cudaSuccess) return e;
-    moe_sort_kernel<<<SORT_CTAS, SORT_WARPS * 32, (size_t)(SORT_WARPS + 2) * p.E * 4, s>>>(p.ids, p.ids64, p.place, p.counts, N, (int)p.E);
-    count_launch();
-    e = cudaGetLastError();
+#define MS(B) launch_sort<B>(p, N, s)
+    cudaError_t e = p.E < 16 ? MS(4) : (p.E < 128 ? MS(7) : (p.E < 512 ? MS(9) : MS(11)));
+#undef MS
     if (e != cudaSuccess || (units == 0 && p.S == 0)) return e;
     const int64_t segs = units > 128 ? (units + 127) / 128 : 1, ctas = (p.T * segs + 7) / 8;
     if (ctas > 0x7fffffffLL) return cudaErrorInvalidValue;

@@ -302,7 +302,7 @@ def routing(g, T, k, E, away=0.0):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32, F8, torch.int8])
 @pytest.mark.parametrize("case", [(1, 1, 1, 16), (1, 8, 64, 4096), (5, 2, 3, 33), (64, 8, 256, 130), (300, 4, 1024, 1024), (1000, 6, 60, 72), (0, 2, 4, 64), (7, 64, 100, 48),
-                                  (257, 33, 40, 4100), (3000, 8, 7, 16)])
+                                  (257, 33, 40, 4100), (3000, 8, 7, 16), (9001, 8, 60, 16)])
 def test_permute(pkg, dev, case, dtype):
     T, k, E, H = case
     g = gen(T + k)

@@ -409,13 +409,11 @@ def block_quant_fp8(x, row_block=1, dtype=None, **kw):
     """x [..., D] f32/f16/bf16 -> (fp8 codes of x's shape, fp32 scales).  One scale per 128 columns of a row
     ([..., ceil(D/128)]), or with row_block=128 per 128 x 128 block of the matrix x ([ceil(rows/128), ceil(D/128)])."""
     import torch
-    q = torch.empty(x.shape, dtype=dtype or torch.float8_e4m3fn, device=x.device)
-    blocks = (x.shape[-1] + 127) // 128
-    if row_block == 1:
-        scale = torch.empty(x.shape[:-1] + (blocks,), dtype=torch.float32, device=x.device)
-    else:
-        rows = x.numel() // x.shape[-1] if x.shape[-1] else 0
-        scale = torch.empty(((rows + row_block - 1) // row_block, blocks), dtype=torch.float32, device=x.device)
+    *lead, D = x.shape
+    q = torch.empty_like(x, dtype=dtype or torch.float8_e4m3fn)
+    if row_block != 1:
+        lead = [(x.numel() // max(D, 1) + row_block - 1) // row_block if row_block > 0 else 0]
+    scale = x.new_empty((*lead, (D + 127) // 128), dtype=torch.float32)
     _run("aclnnB200BlockQuantFp8", x, row_block, q, scale, **kw)
     return q, scale
 
@@ -423,9 +421,10 @@ def block_quant_fp8(x, row_block=1, dtype=None, **kw):
 def swiglu_block_quant_fp8(x, dtype=None, **kw):
     """x [..., 2D] f32/f16/bf16 -> (fp8 codes [..., D] of silu(x[..., :D]) * x[..., D:], fp32 scales [..., ceil(D/128)])."""
     import torch
-    D = x.shape[-1] // 2
-    q = torch.empty(x.shape[:-1] + (D,), dtype=dtype or torch.float8_e4m3fn, device=x.device)
-    scale = torch.empty(x.shape[:-1] + ((D + 127) // 128,), dtype=torch.float32, device=x.device)
+    *lead, D = x.shape
+    D //= 2
+    q = x.new_empty((*lead, D), dtype=dtype or torch.float8_e4m3fn)
+    scale = x.new_empty((*lead, (D + 127) // 128), dtype=torch.float32)
     _run("aclnnB200SwiGluBlockQuantFp8", x, q, scale, **kw)
     return q, scale
 
@@ -434,7 +433,7 @@ def block_quant_matmul(x, x_scale, w, w_scale, transposed=False, out_dtype=None,
     """x fp8 [M,K] with x_scale [M, ceil(K/128)]; w fp8 [K,N] (transposed: [N,K]) with a scale per 128 x 128 block."""
     import torch
     if out is None:
-        out = torch.empty((x.shape[0], w.shape[0 if transposed else 1]), dtype=out_dtype or torch.bfloat16, device=x.device)
+        out = x.new_empty((x.shape[0], w.shape[0 if transposed else 1]), dtype=out_dtype or torch.bfloat16)
     _run("aclnnB200BlockQuantMatmul", x, x_scale, w, w_scale, bool(transposed), out, **kw)
     return out
 
@@ -444,9 +443,8 @@ def block_quant_grouped_matmul(x, x_scale, w, w_scale, rows_per_expert, transpos
     last expert's are left as they were."""
     import torch
     if out is None:
-        out = torch.empty((x.shape[0], w.shape[1 if transposed else 2]), dtype=out_dtype or torch.bfloat16, device=x.device)
-    _run("aclnnB200BlockQuantGroupedMatmul", x, x_scale, w, w_scale, rows_per_expert,
-         bool(transposed), out, **kw)
+        out = x.new_empty((x.shape[0], w.shape[1 if transposed else 2]), dtype=out_dtype or torch.bfloat16)
+    _run("aclnnB200BlockQuantGroupedMatmul", x, x_scale, w, w_scale, rows_per_expert, bool(transposed), out, **kw)
     return out
 
 
@@ -456,30 +454,26 @@ def moe_token_permute(tokens, expert_ids, num_experts, scales=None, out=None, sc
     last one are left as they were in `out` / `scales_out`."""
     import torch
     T, k = expert_ids.shape
-    dev = tokens.device
     if out is None:
-        out = torch.empty((T * k, tokens.shape[1]), dtype=tokens.dtype, device=dev)
+        out = tokens.new_empty((T * k, tokens.shape[1]))
     if scales is not None and scales_out is None:
-        scales_out = torch.empty((out.shape[0], scales.shape[1]), dtype=torch.float32, device=dev)
-    place = torch.empty((T, k), dtype=torch.int32, device=dev)
-    counts = torch.empty((num_experts,), dtype=torch.int64, device=dev)
-    _run("aclnnB200MoeTokenPermute", tokens, expert_ids, scales, out, scales_out, place,
-         counts, **kw)
+        scales_out = scales.new_empty((out.shape[0], scales.shape[1]))
+    place = tokens.new_empty((T, k), dtype=torch.int32)
+    counts = tokens.new_empty((num_experts,), dtype=torch.int64)
+    _run("aclnnB200MoeTokenPermute", tokens, expert_ids, scales, out, scales_out, place, counts, **kw)
     return (out, place, counts) if scales is None else (out, place, counts, scales_out)
 
 
 def moe_token_permute_grad(grad_rows, place, **kw):
     """The gradient of moe_token_permute's tokens: the sum of each token's rows of grad_rows."""
-    import torch
-    out = torch.empty((place.shape[0], grad_rows.shape[1]), dtype=grad_rows.dtype, device=grad_rows.device)
+    out = grad_rows.new_empty((place.shape[0], grad_rows.shape[1]))
     _run("aclnnB200MoeTokenPermuteGrad", grad_rows, place, out, **kw)
     return out
 
 
 def moe_token_unpermute(rows, place, probs=None, **kw):
     """rows [R,H], place int32 [T,k], probs [T,k] -> out [T,H]: the weighted sum of each token's rows."""
-    import torch
-    out = torch.empty((place.shape[0], rows.shape[1]), dtype=rows.dtype, device=rows.device)
+    out = rows.new_empty((place.shape[0], rows.shape[1]))
     _run("aclnnB200MoeTokenUnpermute", rows, place, probs, out, **kw)
     return out
 

@@ -117,6 +117,37 @@ __device__ __forceinline__ void cp_async4(uint32_t dst, const float *src) {
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t local, uint32_t cta) {
+    uint32_t a;
+    float4 v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(local), "r"(cta));
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
+    return v;
+}
+// Four sums of a row to columns n .. n + 3 of out (element `at` is column n; n a multiple of 4).
+__device__ __forceinline__ void store_quad(const BmParams &p, int64_t at, int n, const float4 &v) {
+    if (p.vec_out && n < p.N) {                           // N a multiple of 8, 16-byte aligned
+        if (p.out_type == ET_F32) {
+            *reinterpret_cast<float4 *>((float *)p.out + at) = v;
+        } else {
+            uint2 w;
+            if (p.out_type == ET_BF16) {
+                __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
+                w = make_uint2(*reinterpret_cast<uint32_t *>(&a), *reinterpret_cast<uint32_t *>(&b));
+            } else {
+                __half2 a = __floats2half2_rn(v.x, v.y), b = __floats2half2_rn(v.z, v.w);
+                w = make_uint2(*reinterpret_cast<uint32_t *>(&a), *reinterpret_cast<uint32_t *>(&b));
+            }
+            *reinterpret_cast<uint2 *>((uint16_t *)p.out + at) = w;
+        }
+        return;
+    }
+    if (n < p.N) store_from_float(p.out, p.out_type, at, v.x);
+    if (n + 1 < p.N) store_from_float(p.out, p.out_type, at + 1, v.y);
+    if (n + 2 < p.N) store_from_float(p.out, p.out_type, at + 2, v.z);
+    if (n + 3 < p.N) store_from_float(p.out, p.out_type, at + 3, v.w);
+}
+
 // The table of a launch, filled by one warp: rows of expert e are row_start[e] .. row_start[e + 1], its tiles end at
 // tile_end[e].  Without counts there is one expert with all M rows.
 template <int ROW_TILE>

@@ -11,9 +11,13 @@
 // scales that are there before the block, and a hand-back before the last multiply-adds.  (Sixteen warps with half the columns
 // each fold sooner but issue more: 143 instructions a warp and block, 570 a scheduler against 512 cycles of products.)
 //
+// Fewer tiles than pairs of SMs: a cluster of 2 or 4 pairs cuts K and adds its parts through distributed shared memory.
+//
 // Roles per CTA: warp 0 = TMA producer of its own halves; warp 1 = in the leader the MMA issuer, in the other CTA the relay
 // that tells the leader its stage is filled; warp 2 = scales; warps 4-11 = epilogue.  Waits are bounded, and the pair meets at a cluster
 // barrier before either CTA's memory goes away.
+#include <algorithm>
+
 #include "block_mm_common.cuh"
 
 namespace qmm {
@@ -39,10 +43,10 @@ __device__ __forceinline__ void bp_mma(uint32_t d_tmem, uint64_t a_desc, uint64_
         "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
         ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
 }
-// Arrives on the barrier at this offset in both CTAs when the products issued so far are done.
-__device__ __forceinline__ void bp_commit(uint32_t bar) {
+// Arrives on the barrier at this offset in both CTAs (`pair`: a bit each) when the products issued so far are done.
+__device__ __forceinline__ void bp_commit(uint32_t bar, uint16_t pair) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-                 ::"r"(bar), "h"((uint16_t)3) : "memory");
+                 ::"r"(bar), "h"(pair) : "memory");
 }
 __device__ __forceinline__ uint32_t bp_at(uint32_t addr, uint32_t cta) {
     uint32_t a;
@@ -95,6 +99,35 @@ __device__ __forceinline__ void store_rows(const uint64_t (&acc)[64], uint4 *box
     }
 }
 
+// Sums of SPLIT pairs, in order: this pair's share of the columns, 4 a lane, all of a lane's reads in flight at once (four at a
+// time, each some 1000 cycles, took 9 us of a 17 us call).
+template <int SPLIT>
+__device__ __forceinline__ void join_pairs(const BmParams &p, uint32_t sums, uint32_t pitch, int crank, int ew, int m0, int rows, int n0) {
+    constexpr int SHARE = BP_COLS / SPLIT, PER_ROW = SHARE / 4, AT_ONCE = 32 / PER_ROW, ROWS = 128 / (BP_EPI * AT_ONCE);
+    const int lane = threadIdx.x & 31, col = (crank >> 1) * SHARE + (lane % PER_ROW) * 4, n = n0 + col, r0 = ew * AT_ONCE + lane / PER_ROW;
+    float4 v[SPLIT][ROWS];
+#pragma unroll
+    for (int j = 0; j < SPLIT; ++j) {
+        const uint32_t from = bp_at(sums + (uint32_t)col * 4u, (uint32_t)(2 * j + (crank & 1)));
+#pragma unroll
+        for (int u = 0; u < ROWS; ++u) {
+            const int r = r0 + u * BP_EPI * AT_ONCE;
+            v[j][u] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (r < rows)
+                asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                             : "=f"(v[j][u].x), "=f"(v[j][u].y), "=f"(v[j][u].z), "=f"(v[j][u].w) : "r"(from + (uint32_t)r * pitch) : "memory");
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < ROWS; ++u) {
+        const int r = r0 + u * BP_EPI * AT_ONCE;
+        float4 t = v[0][u];
+#pragma unroll
+        for (int j = 1; j < SPLIT; ++j) { t.x += v[j][u].x; t.y += v[j][u].y; t.z += v[j][u].z; t.w += v[j][u].w; }
+        if (r < rows) store_quad(p, (int64_t)(m0 + r) * p.N + n, n, t);
+    }
+}
+
 __global__ void __launch_bounds__(BP_THREADS, 1)
 block_mm_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w, const BmParams p, const uint32_t idesc) {
     using S = BpSmem;
@@ -112,7 +145,9 @@ block_mm_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
     volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(gen_base + S::MISC_OFF);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(gen_base + S::MISC_OFF + 4);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int rank = (int)blockIdx.x & 1;
+    // a cluster is `split` pairs, each with its part of a tile's k blocks
+    const int crank = (int)blockIdx.x % (2 * p.split), rank = crank & 1, leader = crank & ~1;
+    const int kb0 = (int)((long long)p.nkb * (crank >> 1) / p.split), kb1 = (int)((long long)p.nkb * ((crank >> 1) + 1) / p.split);
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < BP_STAGES; ++s) { mbar_init(bar_full(s), rank == 0 ? 2 : 1); mbar_init(bar_empty(s), 2); }
@@ -134,7 +169,8 @@ block_mm_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
     const int tiles = tile_end[p.E - 1];
-    const int first = (int)blockIdx.x >> 1, step = (int)gridDim.x >> 1;
+    const int first = (int)blockIdx.x / (2 * p.split), step = (int)gridDim.x / (2 * p.split);
+    const bool joined = p.split > 1 && first < tiles;     // one tile per cluster then, summed over its pairs at the end
     TileWalk<BP_ROWS, BP_COLS> walk{row_start, tile_end};
     // The epilogue needs 128 sums and two loads of 32 in registers: the first four warps give up what they do not use.
     // (384 threads x 168 at launch = 128 x 56 + 256 x 224.)
@@ -151,7 +187,7 @@ block_mm_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
             walk.seek(tile, e, m0, rows, n0);
             m0 += rank * 128;
             n0 += rank * 128;
-            for (int kb = 0; kb < p.nkb; ++kb) {
+            for (int kb = kb0; kb < kb1; ++kb) {
                 if (!warp_wait(bar_empty(s), ph, abort_flag, 0x611u)) { ok = false; break; }
                 if (elect_one()) {
                     mbar_expect_tx(bar_full(s), S::STAGE);
@@ -170,12 +206,13 @@ block_mm_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
         const int h = warp >> 1;
         const uint32_t w_step = p.w_nk ? 32u : 4096u, w_lbo = p.w_nk ? 16u : 16384u, w_half = p.w_nk ? 8192u : 64u;
         const uint64_t x_desc = smem_desc(x_tile(0), 16, 1024), w_desc = smem_desc(w_tile(0) + (uint32_t)h * w_half, w_lbo, 1024);
-        const uint32_t peer_full = bp_at(bar_full(0), 0);
+        const uint32_t peer_full = bp_at(bar_full(0), leader);
+        const uint16_t pair = (uint16_t)(3u << leader);
         int s = 0, a = 0;
         uint32_t ph = 0, aph = 1;
         bool ok = true;
         for (int tile = first; tile < tiles && ok; tile += step) {
-            for (int kb = 0; kb < p.nkb; ++kb) {
+            for (int kb = kb0; kb < kb1; ++kb) {
                 if (rank == 0) {
                     if (!warp_wait<true>(bar_full(s), ph, abort_flag, 0x613u) || !warp_wait<true>(bar_acc_empty(h, a), aph, abort_flag, 0x612u)) { ok = false; break; }
                     tc_fence_after();
@@ -184,8 +221,8 @@ block_mm_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
                     if (elect_one()) {
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk) bp_mma(d, xd + (uint32_t)(kk * 2), wd + kk * (w_step >> 4), idesc, kk > 0 ? 1u : 0u);
-                        bp_commit(bar_acc_full(h, a));
-                        bp_commit(bar_empty(s));
+                        bp_commit(bar_acc_full(h, a), pair);
+                        bp_commit(bar_empty(s), pair);
                     }
                     __syncwarp();
                     ++issued;
@@ -203,13 +240,13 @@ block_mm_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
         // scales: the copies run SC_AHEAD blocks in front of the reports.  Slots are reused 16 blocks later, and a report
         // for block i waits for block i - 2 to be complete, by when block i - 4 has been folded.
         TileWalk<BP_ROWS, BP_COLS> ahead{row_start, tile_end};
-        int atile = first, akb = 0, slot = 0, rows = 0;
+        int atile = first, akb = kb0, slot = 0, rows = 0;
         const float *xsp[4], *wsp[2];
         const int ws_step = p.w_nk ? 1 : p.nb;
         bool w_ok = false;
         auto copy_next = [&] {                            // one commit group per block, empty behind the last tile
-            if (atile < tiles) {
-                if (akb == 0) {
+            if (atile < tiles && kb0 < kb1) {
+                if (akb == kb0) {
                     int e, m0, n0;
                     ahead.seek(atile, e, m0, rows, n0);
                     rows -= rank * 128;
@@ -224,7 +261,7 @@ block_mm_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
                 for (int i = 0; i < 4; ++i)
                     if (lane + 32 * i < rows) cp_async4(dst + (lane + 32 * i) * 4, xsp[i] + akb);
                 if (w_ok) cp_async4(dst + (128 + lane) * 4, wsp[0] + (int64_t)akb * ws_step);
-                if (++akb == p.nkb) { akb = 0; atile += step; }
+                if (++akb == kb1) { akb = kb0; atile += step; }
                 slot = (slot + 1) & (SC_SLOTS - 1);
             }
             cp_async_commit();
@@ -234,7 +271,7 @@ block_mm_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
         uint32_t ph = 1;                                  // of the accumulator's previous use
         bool ok = true;
         for (int tile = first; tile < tiles && ok; tile += step) {
-            for (int kb = 0; kb < p.nkb; ++kb) {
+            for (int kb = kb0; kb < kb1; ++kb) {
                 if (!warp_wait(bar_acc_full(0, a), ph, abort_flag, 0x617u) || !warp_wait(bar_acc_full(1, a), ph, abort_flag, 0x618u)) { ok = false; break; }
                 copy_next();
                 cp_async_wait<SC_AHEAD>();
@@ -246,20 +283,24 @@ block_mm_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
         }
         cp_async_wait<0>();
     }
+    if (joined) {                                         // the epilogue's two meetings
+        bm_cluster_sync();
+        bm_cluster_sync();
+    }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         const int ew = warp - 4, h = ew >> 2, q = warp & 3;   // h: this warp's half
         constexpr int COLS = BP_COLS / 2, CH = 32, NCH = COLS / CH;
         const uint32_t tm_lane = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(h * COLS);
-        const uint32_t give = bp_at(bar_acc_empty(h, 0), 0);   // in the leader, of accumulator 0; 8 bytes on, of 1
+        const uint32_t give = bp_at(bar_acc_empty(h, 0), leader);   // in the leader, of accumulator 0; 8 bytes on, of 1
         int a = 0, slot = 0;
         uint32_t ph = 0;
         bool ok = true;
+        uint64_t acc[COLS / 2];
         for (int tile = first; tile < tiles && ok; tile += step) {
-            uint64_t acc[COLS / 2];
 #pragma unroll
             for (int i = 0; i < COLS / 2; ++i) acc[i] = 0ull;
-            for (int kb = 0; kb < p.nkb; ++kb) {
+            for (int kb = kb0; kb < kb1; ++kb) {
                 if (!warp_wait(bar_acc_full(h, a), ph, abort_flag, 0x616u)) { ok = false; break; }
                 tc_fence_after();
                 const uint32_t taddr = tm_lane + (uint32_t)(a * BP_COLS);
@@ -286,7 +327,7 @@ block_mm_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
                 a ^= 1;
                 if (a == 0) ph ^= 1u;
             }
-            if (!ok) break;
+            if (!ok || joined) break;
             int e, m0, rows, n0;
             walk.seek(tile, e, m0, rows, n0);
             m0 += rank * 128 + q * 32;                    // this warp's rows
@@ -311,6 +352,26 @@ block_mm_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
             }
             __syncwarp();
         }
+        if (joined) {
+            // Every pair's sums go to its ring, a row of 256 columns every 1040 bytes (rows in turn start 16 bytes apart in the
+            // banks), once both halves' products have read it ...
+            constexpr uint32_t PITCH = BP_COLS * 4 + 16;
+            static_assert(128 * PITCH <= (uint32_t)S::TABLE_OFF, "the sums fit the ring");
+            asm volatile("bar.sync 1, %0;" ::"n"(BP_EPI * 32) : "memory");
+            uint8_t *mine = gen_base + (uint32_t)(q * 32 + lane) * PITCH + (uint32_t)h * 256u;
+#pragma unroll
+            for (int i = 0; i < COLS / 2; i += 2)
+                *reinterpret_cast<ulonglong2 *>(mine + 8 * i + (i >= COLS / 4 ? 256 : 0)) = make_ulonglong2(acc[i], acc[i + 1]);
+            bm_cluster_sync();
+            // ... and each pair adds its share of the columns over the pairs.
+            int e, m0, rows, n0;
+            walk.seek(first, e, m0, rows, n0);
+            m0 += rank * 128;
+            rows -= rank * 128;
+            if (p.split == 2) join_pairs<2>(p, base, PITCH, crank, ew, m0, rows, n0);
+            else join_pairs<4>(p, base, PITCH, crank, ew, m0, rows, n0);
+            bm_cluster_sync();                            // a CTA's shared memory outlives the others' reads
+        }
     }
 
     tc_fence_before();
@@ -331,7 +392,7 @@ block_mm_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
 
 }  // namespace
 
-cudaError_t launch_block_mm_pair(const BlockMmArgs &a, cudaStream_t s) {
+cudaError_t launch_block_mm_pair(const BlockMmArgs &a, int split, cudaStream_t s) {
     const int E = a.experts > 0 ? (int)a.experts : 1;
     CUtensorMap tx, tw;
     bool ok = make_map(&tx, a.x, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.K, a.M, a.K, BM_BK, 128, CU_TENSOR_MAP_SWIZZLE_128B);
@@ -341,15 +402,15 @@ cudaError_t launch_block_mm_pair(const BlockMmArgs &a, cudaStream_t s) {
     p.xs = a.xs; p.ws = a.ws; p.counts = a.experts > 0 ? a.group_rows : nullptr; p.out = a.out; p.out_type = a.out_type;
     p.vec_out = a.N % 8 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
     p.M = (int)a.M; p.N = (int)a.N; p.nkb = (int)((a.K + BM_BK - 1) / BM_BK); p.nb = (int)((a.N + 127) / 128); p.E = E;
-    p.n_tiles = (int)((a.N + BP_COLS - 1) / BP_COLS); p.w_nk = a.w_nk; p.split = 1;
+    p.n_tiles = (int)((a.N + BP_COLS - 1) / BP_COLS); p.w_nk = a.w_nk; p.split = split;
     const uint32_t idesc = bm_idesc(a.x_type == ET_E5M2, a.w_type == ET_E5M2, 0, a.w_nk ? 0 : 1, BP_ROWS, BP_COLS / 2);
     // tiles: each expert with rows adds at most one partly filled row tile
     const int64_t full = (a.M + BP_ROWS - 1) / BP_ROWS, most = a.experts > 0 ? (a.M < full + E - 1 ? a.M : full + E - 1) : full;
-    const int64_t tiles = most * p.n_tiles, pairs = sm_count() / 2;
+    const int64_t tiles = most * p.n_tiles, pairs = split > 1 ? tiles * split : std::min<int64_t>(tiles, sm_count() / 2);
     cudaError_t e = allow_smem<block_mm_pair_kernel>(BpSmem::TOTAL);
     if (e != cudaSuccess) return e;
     if (!has_regs<block_mm_pair_kernel>(168)) return cudaErrorInvalidConfiguration;
-    e = launch_chained(block_mm_pair_kernel, 2 * (unsigned)(tiles < pairs ? tiles : pairs), BP_THREADS, BpSmem::TOTAL, 2, s, tx, tw, p, idesc);
+    e = launch_chained(block_mm_pair_kernel, (unsigned)(2 * pairs), BP_THREADS, BpSmem::TOTAL, (unsigned)(2 * split), s, tx, tw, p, idesc);
     if (e == cudaSuccess) count_launch();
     return e;
 }

@@ -50,14 +50,6 @@ __device__ __forceinline__ void bm_mma(uint32_t d_tmem, uint64_t a_desc, uint64_
         "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
         ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
 }
-__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t local, uint32_t cta) {
-    uint32_t a;
-    float4 v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(local), "r"(cta));
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
-    return v;
-}
-
 template <int NT>
 __global__ void __launch_bounds__(BT_THREADS, 1)
 block_mm_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w, const BmParams p, const uint32_t idesc) {
@@ -164,7 +156,7 @@ block_mm_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
             const float *xsp = p.xs, *wsp = p.ws;
             const int ws_step = p.w_nk ? 1 : p.nb;
             auto copy_next = [&] {                        // one commit group per call, empty behind the last tile
-                if (atile < tiles) {
+                if (atile < tiles && g0 < g1) {
                     if (ag == g0) {
                         int e, m0, n0;
                         ahead.seek(atile, e, m0, rows, n0);
@@ -295,11 +287,7 @@ block_mm_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
                 for (int c = 1; c < 8; ++c)
                     if (c < p.split) { v.x += part[c].x; v.y += part[c].y; v.z += part[c].z; v.w += part[c].w; }
                 const int n = n0 + lane * 4;
-                const int64_t at = (int64_t)(m0 + r) * p.N + n;
-                if (n < p.N) store_from_float(p.out, p.out_type, at, v.x);
-                if (n + 1 < p.N) store_from_float(p.out, p.out_type, at + 1, v.y);
-                if (n + 2 < p.N) store_from_float(p.out, p.out_type, at + 2, v.z);
-                if (n + 3 < p.N) store_from_float(p.out, p.out_type, at + 3, v.w);
+                store_quad(p, (int64_t)(m0 + r) * p.N + n, n, v);
             }
         }
         bm_cluster_sync();                                // a CTA's shared memory outlives the others' reads
@@ -330,6 +318,7 @@ template <int NT> cudaError_t launch_form(const BlockMmArgs &a, int split, cudaS
     BmParams p{};
     p.xs = a.xs; p.ws = a.ws; p.counts = a.experts > 0 ? a.group_rows : nullptr; p.out = a.out; p.out_type = a.out_type;
     p.M = (int)a.M; p.N = (int)a.N; p.nkb = (int)((a.K + BM_BK - 1) / BM_BK); p.nb = (int)((a.N + 127) / 128); p.E = E;
+    p.vec_out = a.N % 8 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
     p.n_tiles = (int)((a.N + BM_LANES - 1) / BM_LANES); p.w_nk = a.w_nk; p.split = split;
     const uint32_t idesc = bm_idesc(a.w_type == ET_E5M2, a.x_type == ET_E5M2, a.w_nk ? 0 : 1, 0, BM_LANES, NT);
     // tiles: each expert with rows adds at most one partly filled row tile
@@ -353,10 +342,12 @@ bool block_mm_tc_supported(const BlockMmArgs &a) {
 }
 
 // The form with the least estimated time.  Rounds of tiles over the SMs x the measured time of a step of K: 0.62, 0.78
-// and 1.0 us per group of two blocks with 16, 32 and 64 rows a tile, 0.5 us per block and pair of CTAs with 256 x 256 tiles.
-// (Microseconds, this form / pairs: 64 x 4096 x 14336 18.7 / 18.8, 128 x 4096 x 14336 29.9 / 19.8, 128 x 4096 x 4096 11.8 / 16.6,
-// 77 x 4112 x 2000 9.7 / 17; 64 experts, 2048 x 2816, 16 rows each 64 / 81, 32 rows 84 / 88, 64 rows 126 / 91.  A form with 128 rows a
-// tile was never the fastest.)  The rows of an expert are not known here: their mean stands in, with half a tile more per expert.
+// and 1.0 us per group of two blocks with 16, 32 and 64 rows a tile (1 us more where a cluster cuts K), 0.42 us per block and pair
+// of CTAs with 256 x 256 tiles (6 or 9 us more for a K cut by 2 or 4: the meeting, 128 KB of sums written and read back).
+// Microseconds, this form / pairs / pairs with K cut by 2: 64 x 4096 x 14336 18.7 / 18.8 / -, 128 x 4096 x 14336 29.9 / 19.8 / -,
+// 128 x 4096 x 4096 11.8 / 16.9 / 16.6, 77 x 4112 x 2000 9.7 / 17 / -, 256 x 14336 x 4096 - / 44.8 / 31.3; 64 experts, 2048 x 2816, 16 rows
+// each 64 / 81, 32 rows 84 / 88, 64 rows 126 / 91.  A form with 128 rows a tile was never the fastest.
+// The rows of an expert are not known here: their mean stands in, with half a tile more per expert.
 cudaError_t launch_block_mm_tc(const BlockMmArgs &a, cudaStream_t s) {
     const int64_t nkb = (a.K + BM_BK - 1) / BM_BK, groups = (nkb + 1) / 2, sms = sm_count();
     const double experts = a.experts > 0 ? (double)std::min(a.experts, a.M) : 1.0, mean = (double)a.M / experts;
@@ -364,16 +355,24 @@ cudaError_t launch_block_mm_tc(const BlockMmArgs &a, cudaStream_t s) {
         const double per = a.experts > 0 ? std::max(1.0, mean / tile_rows + 0.5) : std::ceil(mean / tile_rows);
         return experts * per * (double)((a.N + tile_cols - 1) / tile_cols) / slots;
     };
-    double best = std::ceil(rounds(256, 256, (double)(sms / 2))) * (double)nkb * 0.5;
+    // the most tiles there can be, whatever the experts' rows: a cluster that cuts K has one tile
+    auto most = [&](int tile_rows, int tile_cols) {
+        const int64_t full = (a.M + tile_rows - 1) / tile_rows;
+        return (a.experts > 0 ? std::min<int64_t>(a.M, full + a.experts - 1) : full) * ((a.N + tile_cols - 1) / tile_cols);
+    };
     int best_nt = 0, best_split = 1;
+    double best = std::ceil(rounds(256, 256, (double)(sms / 2))) * (double)nkb * 0.42;
+    for (int split = 2; split <= 4; split *= 2) {
+        // clusters of 4 and 8 CTAs: 33 and 15 of them fit 148 SMs at once
+        if ((double)most(256, 256) > (double)sms / (split == 2 ? 4.5 : 9.9) || split * 8 > nkb) break;
+        const double t = (double)((nkb + split - 1) / split) * 0.42 + (split == 2 ? 6.0 : 9.0);
+        if (t < best) { best = t; best_split = split; }
+    }
     const int nts[3] = {16, 32, 64};
     const double step_us[3] = {0.62, 0.78, 1.0};
     for (int i = 0; i < 3; ++i) {
-        // a cluster's CTAs have one tile, so a split has to fit the SMs at once, for every distribution of the rows
-        const int64_t full = (a.M + nts[i] - 1) / nts[i], cols = (a.N + BM_LANES - 1) / BM_LANES;
-        const int64_t most = (a.experts > 0 ? std::min<int64_t>(a.M, full + a.experts - 1) : full) * cols;
         int split = 1;
-        while (split < 8 && most * split * 2 <= sms && split * 4 <= groups) split *= 2;
+        while (split < 8 && most(nts[i], BM_LANES) * split * 2 <= sms && split * 4 <= groups) split *= 2;
         const double t = std::ceil(rounds(nts[i], BM_LANES, (double)sms) * split) * (double)((groups + split - 1) / split) * step_us[i] + (split > 1 ? 1.0 : 0.0);
         if (t < best) { best = t; best_nt = nts[i]; best_split = split; }
     }
@@ -381,7 +380,7 @@ cudaError_t launch_block_mm_tc(const BlockMmArgs &a, cudaStream_t s) {
         case 16: return launch_form<16>(a, best_split, s);
         case 32: return launch_form<32>(a, best_split, s);
         case 64: return launch_form<64>(a, best_split, s);
-        default: return launch_block_mm_pair(a, s);
+        default: return launch_block_mm_pair(a, best_split, s);
     }
 }
 

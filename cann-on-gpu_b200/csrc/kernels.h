@@ -159,7 +159,8 @@ cudaError_t launch_block_mm_tc(const BlockMmArgs &p, cudaStream_t s);
 unsigned int block_mm_device_status();
 void block_mm_device_status_reset();
 // The same for many rows: pairs of CTAs (block_mm_pair.cu).
-cudaError_t launch_block_mm_pair(const BlockMmArgs &p, cudaStream_t s);
+// `split` pairs share a tile (1, 2 or 4; above 1 all tiles x split have to be worth a launch of their own).
+cudaError_t launch_block_mm_pair(const BlockMmArgs &p, int split, cudaStream_t s);
 unsigned int block_mm_pair_device_status();
 void block_mm_pair_device_status_reset();
 

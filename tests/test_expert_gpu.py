@@ -242,9 +242,45 @@ def test_block_matmul_unaligned_pointers(pkg, dev, M):
         within(out, want, mm_tol(want, mag, K, torch.bfloat16))
 
 
+def mm_ref_on(dev, x, xs, w, ws, nk):
+    """mm_ref computed on the device, for sizes that take the CPU seconds."""
+    want, mag = mm_ref(x.to(dev), xs.to(dev), w.to(dev), ws.to(dev), nk)
+    return want.cpu(), mag.cpu()
+
+
+# few wide tiles and a long K: the sums of a tile come from 2 or 4 pairs of CTAs (251 rows), or 2 to 8 CTAs (others)
+@pytest.mark.parametrize("shape", [(250, 14320, 4080, True), (251, 8176, 2032, False), (251, 8176, 2040, True), (130, 14336, 4096, False), (60, 4096, 1000, True),
+                                   (9, 7184, 264, True)])
+def test_block_matmul_cut_along_k(pkg, dev, shape):
+    M, K, N, nk = shape
+    g = gen(M)
+    x, xs = codes(g, M, K, F8)
+    w, ws = weights(g, 1, K, N, nk)
+    want, mag = mm_ref_on(dev, x, xs, w[0], ws[0], nk)
+    for dtype in (torch.bfloat16, torch.float32):
+        args = (x.to(dev), xs.to(dev), w[0].to(dev), ws[0].to(dev))
+        out = pkg.block_quant_matmul(*args, transposed=nk, out_dtype=dtype)
+        within(out, want, mm_tol(want, mag, K, dtype), f"{shape} {dtype}")
+        assert torch.equal(out, pkg.block_quant_matmul(*args, transposed=nk, out_dtype=dtype))      # the parts meet in order
+
+
+# more tiles than SMs, rows and columns ending inside them
+@pytest.mark.parametrize("shape", [(2500, 528, 5000, True), (1100, 1040, 12304, False), (33, 272, 30000, True)])
+def test_block_matmul_many_tiles(pkg, dev, shape):
+    M, K, N, nk = shape
+    g = gen(N)
+    x, xs = codes(g, M, K, F8)
+    w, ws = weights(g, 1, K, N, nk)
+    want, mag = mm_ref_on(dev, x, xs, w[0], ws[0], nk)
+    for dtype in (torch.float16, torch.float32):
+        out = pkg.block_quant_matmul(x.to(dev), xs.to(dev), w[0].to(dev), ws[0].to(dev), transposed=nk, out_dtype=dtype)
+        within(out, want, mm_tol(want, mag, K, dtype), f"{shape} {dtype}")
+
+
 GROUPS = {
     "even": [40, 40, 40, 40], "ragged": [1, 0, 129, 77, 0, 3, 256, 128, 5], "one": [0, 0, 300, 0], "none": [0, 0, 0], "behind": [10, 20, 0],
-    "many": [i % 5 for i in range(67)], "single": [1] * 40, "large": [700, 3, 513],
+    "many": [i % 5 for i in range(67)], "single": [1] * 40, "large": [700, 3, 513], "most": [3 if i % 7 == 0 else 0 for i in range(1024)],
+    "middle": [90, 0, 200, 17, 64, 33, 255, 1],
 }
 
 

@@ -99,8 +99,7 @@ __device__ __forceinline__ void store_rows(const uint64_t (&acc)[64], uint4 *box
     }
 }
 
-// Sums of SPLIT pairs, in order: this pair's share of the columns, 4 a lane, all of a lane's reads in flight at once (four at a
-// time, each some 1000 cycles, took 9 us of a 17 us call).
+// Sums of SPLIT pairs, in order: this pair's share of the columns, 4 a lane, all of a lane's reads in flight at once.
 template <int SPLIT>
 __device__ __forceinline__ void join_pairs(const BmParams &p, uint32_t sums, uint32_t pitch, int crank, int ew, int m0, int rows, int n0) {
     constexpr int SHARE = BP_COLS / SPLIT, PER_ROW = SHARE / 4, AT_ONCE = 32 / PER_ROW, ROWS = 128 / (BP_EPI * AT_ONCE);

@@ -26,6 +26,13 @@ template <bool E5M2> __device__ __forceinline__ float block_scale(float amax) {
     return amax > 0.f ? fmaxf(__fdiv_rn(amax, top), 1.17549435e-38f) : 1.f;
 }
 
+// a / (1 + exp(-a)) with t = exp(-|a|): a / (1 + t) or a t / (1 + t), so that nothing overflows and the divisor stays in
+// [1, 2], where the fast quotient is good to 2 ulp.
+__device__ __forceinline__ float silu(float a) {
+    const float t = __expf(-fabsf(a));
+    return __fdividef(a < 0.f ? a * t : a, 1.f + t);
+}
+
 // N consecutive elements as fp32 from x[idx] (N * size is 16 or 32 bytes, aligned), or `n` of them one by one.
 template <int T, int N> struct Lane {
     static constexpr int W = N * (T == ET_F32 ? 4 : 2) / 4;
@@ -79,7 +86,7 @@ __global__ void __launch_bounds__(256) block_quant_kernel(const void *x, uint8_t
             float h[N];
             g.widen(h);
 #pragma unroll
-            for (int i = 0; i < N; ++i) f[i] = __fdividef(f[i], 1.f + __expf(-f[i])) * h[i];
+            for (int i = 0; i < N; ++i) f[i] = silu(f[i]) * h[i];
         }
     } else {
         load_each<T, N, LPB>(x, in, left, f);
@@ -87,7 +94,7 @@ __global__ void __launch_bounds__(256) block_quant_kernel(const void *x, uint8_t
             float h[N];
             load_each<T, N, LPB>(x, in + D, left, h);
 #pragma unroll
-            for (int i = 0; i < N; ++i) f[i] = __fdividef(f[i], 1.f + __expf(-f[i])) * h[i];
+            for (int i = 0; i < N; ++i) f[i] = silu(f[i]) * h[i];
         }
     }
 #pragma unroll

@@ -25,11 +25,15 @@ bool sane(const aclTensor *t) {
 int64_t bytes_of(const aclTensor *t) { return t->numel() * (int64_t)dtype_size(t->dtype); }
 char *ptr_of(const aclTensor *t) { return t && t->data ? (char *)t->data + t->offset * (int64_t)dtype_size(t->dtype) : nullptr; }
 
-// 161001 for a missing pointer, 161002 for an output that overlaps another tensor of the call.
+// 161001 for a missing pointer, 161002 for one off its elements' boundary and for an output that overlaps another
+// tensor of the call.
 aclnnStatus check_pointers(std::initializer_list<const aclTensor *> in, std::initializer_list<const aclTensor *> out) {
     for (auto &list : {in, out})
-        for (const aclTensor *t : list)
-            if (t && bytes_of(t) > 0 && !t->data) return ACLNN_ERR_PARAM_NULLPTR;
+        for (const aclTensor *t : list) {
+            if (!t || bytes_of(t) == 0) continue;
+            if (!t->data) return ACLNN_ERR_PARAM_NULLPTR;
+            if (reinterpret_cast<uintptr_t>(ptr_of(t)) % dtype_size(t->dtype) != 0) return ACLNN_ERR_PARAM_INVALID;
+        }
     auto meet = [](const aclTensor *a, const aclTensor *b) {
         if (!a || !b || bytes_of(a) == 0 || bytes_of(b) == 0) return false;
         const char *pa = ptr_of(a), *pb = ptr_of(b);

@@ -156,6 +156,7 @@ def test_phase2_refuses_before_launching(pkg):
     rows, place, probs, out = at([8, 64], B, 0x10000), at([4, 2], I, 0x20000), at([4, 2], F, 0x30000), at([4, 64], B, 0x10100)
     assert run("aclnnB200MoeTokenUnpermute", plan(pkg, "aclnnB200MoeTokenUnpermute", rows, place, probs, out)) == BAD
     assert run("aclnnB200MoeTokenUnpermute", plan(pkg, "aclnnB200MoeTokenUnpermute", rows, place, at([4, 2], F, 0), at([4, 64], B, 0x40000))) == NULL
+    assert run("aclnnB200BlockQuantFp8", plan(pkg, "aclnnB200BlockQuantFp8", x, i64(1), q, at([4, 2], F, 0x30002))) == BAD       # off a float's boundary
     # an empty batch needs no pointers and launches nothing
     assert run("aclnnB200MoeTokenUnpermute", plan(pkg, "aclnnB200MoeTokenUnpermute", at([0, 64], B, 0), at([0, 2], I, 0), None, at([0, 64], B, 0))) == OK
     assert run("aclnnB200BlockQuantMatmul", plan(pkg, "aclnnB200BlockQuantMatmul", at([0, 64], E4, 0), at([0, 1], F, 0), at([64, 32], E4, 0x1000),

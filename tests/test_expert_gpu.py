@@ -433,6 +433,42 @@ def test_unpermute_gradient(pkg, dev, case, dtype):
         within(drows, want, tol, "rows")
 
 
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("H", [40, 33, 2048])
+def test_places_that_name_no_row(pkg, dev, dtype, H):
+    """Places below 0 and behind the last row stand for no row: their weights (NaN here) take no part, their gradients are 0."""
+    T, k, R = 5, 3, 9
+    g = gen(H)
+    place = torch.tensor([[0, -1, 8], [9, 1, -(1 << 31)], [(1 << 31) - 1, 9, -1], [2, 3, 4], [5, 100, 6]], dtype=torch.int32)
+    ok = (place >= 0) & (place < R)
+    rows, dout, probs = torch.randn((R, H), generator=g).to(dtype), torch.randn((T, H), generator=g).to(dtype), torch.rand((T, k), generator=g)
+    nan_probs = torch.where(ok, probs, torch.full_like(probs, float("nan")))
+    want, mag = gather_ref(rows, torch.where(ok, place, torch.full_like(place, -1)), probs * ok)
+    out = pkg.moe_token_unpermute(rows.to(dev), place.to(dev), nan_probs.to(dev))
+    within(out, want, rounding(want, dtype) + (k + 1) * 2.0 ** -23 * mag)
+    assert (out[2] == 0).all()
+    buf = torch.full((R, H), 3.0, dtype=dtype, device=dev)
+    drows, dprobs = pkg.moe_token_unpermute_grad(dout.to(dev), rows.to(dev), place.to(dev), nan_probs.to(dev), out=buf)
+    assert (dprobs.cpu()[~ok] == 0).all() and (drows[7] == 3.0).all() and torch.isfinite(drows).all()
+    v = rows.double()[place.long().clamp(0, R - 1)] * ok[..., None]
+    within(dprobs, (dout.double()[:, None] * v).sum(-1), rounding((dout.double()[:, None] * v).sum(-1), torch.float32) + (H + 8) * 2.0 ** -23 *
+           (dout.double()[:, None] * v).abs().sum(-1))
+
+
+def test_swiglu_far_from_zero(pkg, dev):
+    """Gates whose exponential leaves fp32's range: the value, not 0 or NaN."""
+    a = torch.tensor([-200.0, -100.0, -88.5, -87.4, -50.0, 50.0, 88.5, 100.0, 200.0, 0.0, -0.0])
+    x = torch.zeros((len(a), 256))
+    x[:, 0], x[:, 128] = a, 1e30
+    q, s = pkg.swiglu_block_quant_fp8(x.to(dev))
+    g = a.double() * torch.sigmoid(a.double()) * 1e30
+    got = q[:, 0].double().cpu() * s[:, 0].double().cpu()
+    # the value is the block's maximum, so its code is exact: what is left is the sigmoid's and the scale's rounding
+    # (below 2^-126 the exponential is a subnormal number, off by 2^-149)
+    tol = g.abs() * ((2 * a.double().abs() * 1.4427 + 14) * 2.0 ** -23 + 2.0 ** -24) + a.double().abs() * 2.0 ** -149 * 1e30
+    within(got, g, tol)
+
+
 def test_gradients_against_differences(pkg, dev):
     """Both sums are linear in their rows and weights, so a difference quotient is exact up to rounding."""
     T, k, E, H = 40, 4, 12, 200

@@ -66,6 +66,56 @@ cudaError_t launch_chained(void (*kernel)(P...), unsigned grid, unsigned threads
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
 }
 
+// Launch of clusters of `cluster` CTAs, behind everything before it on the stream.
+template <typename... P, typename... A>
+cudaError_t launch_cluster(void (*kernel)(P...), unsigned grid, unsigned threads, size_t smem, unsigned cluster, cudaStream_t s, A... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cluster > 8) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess) return e;
+    }
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+    if (e == cudaSuccess) count_launch();
+    return e;
+}
+// Whether the current device can hold such a cluster of `Kernel` at all.
+template <auto Kernel> bool cluster_fits(unsigned cluster, unsigned threads, size_t smem) {
+    static std::atomic<int> known[64];   // 0 unknown, 1 no, 2 yes
+    const int dev = current_device();
+    int k = known[dev].load(std::memory_order_relaxed);
+    if (k == 0) {
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(cluster);
+        cfg.blockDim = dim3(threads);
+        cfg.dynamicSmemBytes = smem;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = cluster;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        int n = 0;
+        const bool ok = allow_smem<Kernel>((int)smem) == cudaSuccess &&
+                        cudaFuncSetAttribute(Kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+                        cudaOccupancyMaxActiveClusters(&n, Kernel, &cfg) == cudaSuccess && n > 0;
+        if (!ok) cudaGetLastError();     // the answer is no, and no error of the call to come
+        k = ok ? 2 : 1;
+        known[dev].store(k, std::memory_order_relaxed);
+    }
+    return k == 2;
+}
 // Launch of a kernel whose CTAs step through `work` items: as many as stay resident, at most one per item.
 template <auto Kernel, typename... A> cudaError_t launch_resident(int64_t work, int threads, cudaStream_t s, A... args) {
     static std::atomic<int> known[64][8];   // CTAs per SM by device and warps

@@ -338,7 +338,7 @@ def routing(g, T, k, E, away=0.0):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32, F8, torch.int8])
 @pytest.mark.parametrize("case", [(1, 1, 1, 16), (1, 8, 64, 4096), (5, 2, 3, 33), (64, 8, 256, 130), (300, 4, 1024, 1024), (1000, 6, 60, 72), (0, 2, 4, 64), (7, 64, 100, 48),
-                                  (257, 33, 40, 4100), (3000, 8, 7, 16), (9001, 8, 60, 16)])
+                                  (257, 33, 40, 4100), (3000, 8, 7, 16), (9001, 8, 60, 16), (1100, 3, 1023, 24), (70000, 1, 130, 4)])
 def test_permute(pkg, dev, case, dtype):
     T, k, E, H = case
     g = gen(T + k)
@@ -580,6 +580,44 @@ def test_expert_layer_captured_and_replayed(pkg, dev):
     torch.cuda.synchronize()
     got = a.out.clone()
     assert torch.equal(got, a.run())
+
+
+def test_large_permutes_captured_and_on_two_streams(pkg, dev):
+    """Permutes of many pairs (a sort and a copy): two captured graphs replayed in turns, and two streams at once, keep apart."""
+    cases = []
+    for i, (T, k, E, H) in enumerate(((700, 4, 30, 64), (3000, 2, 256, 40))):
+        g = gen(40 + i)
+        ids = routing(g, T, k, E, 0.1)
+        x = torch.randn((T, H), generator=g).to(torch.bfloat16)
+        cases.append((x.to(dev), ids.int().to(dev), E, torch.zeros((T * k, H), dtype=torch.bfloat16, device=dev)) + route_ref(ids, E))
+    run = lambda c: pkg.moe_token_permute(c[0], c[1], c[2], out=c[3])
+    check = lambda c, got: torch.equal(got[1].cpu(), c[4]) and torch.equal(got[2].cpu(), c[5]) and all(
+        torch.equal(got[0][c[4][t, j]].cpu(), c[0][t].cpu()) for t, j in ((0, 0), (5, 1), (-1, -1)) if c[4][t, j] >= 0)
+    for c in cases:
+        assert check(c, run(c))
+    torch.cuda.synchronize()
+    graphs = []
+    for c in cases:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            got = run(c)
+        graphs.append((g, got))
+    for _ in range(3):
+        for c in cases:
+            c[3].zero_()
+        for g, _ in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        assert all(check(c, got) for c, (_, got) in zip(cases, graphs))
+    streams = [torch.cuda.Stream(dev) for _ in cases]
+    for _ in range(4):
+        outs = []
+        for c, s in zip(cases, streams):
+            s.wait_stream(torch.cuda.current_stream(dev))
+            with torch.cuda.stream(s):
+                outs.append(run(c))
+        torch.cuda.synchronize()
+        assert all(check(c, got) for c, got in zip(cases, outs))
 
 
 def test_two_streams_at_once(pkg, dev):

@@ -153,34 +153,33 @@ __device__ __forceinline__ void store_quad(const BmParams &p, int64_t at, int n,
 template <int ROW_TILE>
 __device__ __forceinline__ void fill_table(const int64_t *counts, int M, int E, int n_tiles, int *row_start, int *tile_end) {
     const int lane = threadIdx.x & 31;
-            if (!counts) {
-                if (lane == 0) { row_start[0] = 0; row_start[1] = M; tile_end[0] = (M + ROW_TILE - 1) / ROW_TILE * n_tiles; }
-            } else {
-                // counts below 0 count as 0, and rows end at M
-                int rows = 0, tiles = 0;
-                for (int e0 = 0; e0 < E; e0 += 32) {
-                    const int e = e0 + lane;
-                    long long c = e < E ? __ldg((const long long *)counts + e) : 0;
-                    c = c < 0 ? 0 : (c > M ? M : c);
-                    long long end = c;
-    #pragma unroll
-                    for (int o = 1; o < 32; o <<= 1) {
-                        const long long v = __shfl_up_sync(0xffffffffu, end, o);
-                        if (lane >= o) end += v;
-                    }
-                    const long long lo64 = rows + end - c, hi64 = rows + end;
-                    const int lo = (int)(lo64 < M ? lo64 : M), hi = (int)(hi64 < M ? hi64 : M);
-                    int t = (hi - lo + ROW_TILE - 1) / ROW_TILE * n_tiles;
-    #pragma unroll
-                    for (int o = 1; o < 32; o <<= 1) {
-                        const int v = __shfl_up_sync(0xffffffffu, t, o);
-                        if (lane >= o) t += v;
-                    }
-                    if (e < E) { row_start[e] = lo; tile_end[e] = tiles + t; if (e == E - 1) row_start[E] = hi; }
-                    rows = __shfl_sync(0xffffffffu, hi, 31);
-                    tiles += __shfl_sync(0xffffffffu, t, 31);
-                }
-            }
+    if (!counts) {
+        if (lane == 0) { row_start[0] = 0; row_start[1] = M; tile_end[0] = (M + ROW_TILE - 1) / ROW_TILE * n_tiles; }
+        return;
+    }
+    int rows = 0, tiles = 0;                              // counts below 0 count as 0, and rows end at M
+    for (int e0 = 0; e0 < E; e0 += 32) {
+        const int e = e0 + lane;
+        long long c = e < E ? __ldg((const long long *)counts + e) : 0;
+        c = c < 0 ? 0 : (c > M ? M : c);
+        long long end = c;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long v = __shfl_up_sync(0xffffffffu, end, o);
+            if (lane >= o) end += v;
+        }
+        const long long lo64 = rows + end - c, hi64 = rows + end;
+        const int lo = (int)(lo64 < M ? lo64 : M), hi = (int)(hi64 < M ? hi64 : M);
+        int t = (hi - lo + ROW_TILE - 1) / ROW_TILE * n_tiles;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, t, o);
+            if (lane >= o) t += v;
+        }
+        if (e < E) { row_start[e] = lo; tile_end[e] = tiles + t; if (e == E - 1) row_start[E] = hi; }
+        rows = __shfl_sync(0xffffffffu, hi, 31);
+        tiles += __shfl_sync(0xffffffffu, t, 31);
+    }
 }
 
 // Tile t in ascending t: expert, first row and rows, first column.

@@ -19,9 +19,11 @@ __device__ __forceinline__ int expert_of(const void *ids, bool ids64, int64_t i,
 }
 
 // ---- the sort: one cluster of 8 or 16 CTAs, no workspace ------------------------------------------------
-// The pairs are cut into contiguous shares, one per warp of the cluster.  Pass 1 counts experts per warp (lanes of one expert find each
-// other by a ballot per bit of the expert's number: 4 instructions each, where match_any took about 270 cycles), then each expert's counts are summed over the warps before, the CTAs before (distributed shared
-// memory) and the experts before; pass 2 walks the shares again and hands out places in order.
+// The pairs are cut into contiguous shares, one per warp of the cluster.  Pass 1 counts experts per warp (lanes of one expert
+// find each other by a ballot per bit of the expert's number: 4 instructions each, where match_any took about 270 cycles),
+// then each expert's counts are summed over the warps before, the CTAs before (distributed shared memory) and the experts
+// before; pass 2 hands out places in order.  What bounds it is that chain of steps, not bytes: 65528 pairs over 256 experts take
+// 8.5 us with 16 CTAs and 11.5 us with 8 (2400 pairs: 5.1 us with either), 128 pairs 2 us in the one-launch form below.
 constexpr int SORT_WARPS = 32;
 
 __device__ __forceinline__ void cluster_arrive() { __syncwarp(); asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }

@@ -17,9 +17,10 @@
  * Common rules.  All tensors are dense (contiguous) in ACL_FORMAT_ND; outputs overlap neither inputs nor each other
  * (161002 at phase 2).  Sizes of zero are allowed where a batch may be empty.  Phase 1 returns 161001 for null arguments and
  * 161002 for unsupported types or shapes; phase 2 returns 161001 for a null data pointer, 161002 for a workspace that
- * is too small, a data pointer off its elements' boundary or a plan of another operator, 361001 for a launch error, and consumes
- * the executor.  Element-aligned is enough for any tensor; 16 or 32 bytes (and row sizes that are multiples of it) get the fast kernels.  Calls keep no state: results do not
- * depend on earlier calls, and the same inputs give the same bits.
+ * is too small, a data pointer off its elements' boundary or a plan of another operator, 361001 for a launch error, and
+ * consumes the executor.  No operator here asks for a workspace.  Element-aligned is enough for any tensor; 16 or 32 bytes
+ * (and row sizes that are multiples of it) get the fast kernels.  Calls keep no state: results do not depend on earlier
+ * calls, and the same inputs give the same bits.
  */
 #ifndef B200_ACLNN_BLOCK_QUANT_MOE_H
 #define B200_ACLNN_BLOCK_QUANT_MOE_H
@@ -54,7 +55,9 @@ B200_ACLNN_RUN(aclnnB200SwiGluBlockQuantFp8)
  * x [M,K] and weight of ACL_FLOAT8_E4M3FN or ACL_FLOAT8_E5M2 (they may differ), xScale ACL_FLOAT [M, ceil(K/128)].
  * transposeWeight false: weight [K,N], weightScale ACL_FLOAT [ceil(K/128), ceil(N/128)]; true: weight [N,K],
  * weightScale [ceil(N/128), ceil(K/128)].  out [M,N]: ACL_BF16, ACL_FLOAT16 or ACL_FLOAT.  Products and sums are fp32,
- * with one rounding to out's type.  K >= 1, N >= 1, M >= 0. */
+ * with one rounding to out's type.  K >= 1, N >= 1, M >= 0.
+ * The gradient of x is the same operator on the quantised gradient of out, with the same weight and weightScale and the
+ * other transposeWeight (also per expert, below).  The weights are codes, so they have no gradient here. */
 ACL_FUNC_VISIBILITY aclnnStatus aclnnB200BlockQuantMatmulGetWorkspaceSize(const aclTensor *x, const aclTensor *xScale,
     const aclTensor *weight, const aclTensor *weightScale, bool transposeWeight, aclTensor *out,
     uint64_t *workspaceSize, aclOpExecutor **executor);

@@ -277,6 +277,33 @@ def test_block_matmul_many_tiles(pkg, dev, shape):
         within(out, want, mm_tol(want, mag, K, dtype), f"{shape} {dtype}")
 
 
+@pytest.mark.parametrize("nk", [False, True])
+@pytest.mark.parametrize("M", [1, 75, 300])
+def test_block_matmul_gradient_of_x(pkg, dev, M, nk):
+    """The gradient of x is the product with the same weight and scales read the other way round, dense and per expert."""
+    K, N, E = 528, 304, 3
+    g = gen(M + 90)
+    w, ws = weights(g, E, K, N, nk)
+    dy, dys = codes(g, M, N, F8E5)
+    dyv = dy.double() * dys.double().repeat_interleave(128, 1)[:, :N]
+    wide = [w[e].double() * ws[e].double().repeat_interleave(128, 0).repeat_interleave(128, 1)[:w.shape[1], :w.shape[2]] for e in range(E)]
+    x = torch.randn((M, K), generator=g, dtype=torch.float64).requires_grad_()
+    rows = [M // 2, 0, M - M // 2]
+    for counts in (None, rows):
+        if counts is None:
+            y = x @ (wide[0].t() if nk else wide[0])
+            mag = dyv.abs() @ (wide[0] if nk else wide[0].t()).abs()
+            got = pkg.block_quant_matmul(dy.to(dev), dys.to(dev), w[0].to(dev), ws[0].to(dev), transposed=not nk, out_dtype=torch.float32)
+        else:
+            parts = torch.split(x, counts)
+            y = torch.cat([v @ (wide[e].t() if nk else wide[e]) for e, v in enumerate(parts)])
+            mag = torch.cat([v.abs() @ (wide[e] if nk else wide[e].t()).abs() for e, v in enumerate(torch.split(dyv, counts))])
+            got = pkg.block_quant_grouped_matmul(dy.to(dev), dys.to(dev), w.to(dev), ws.to(dev), torch.tensor(counts, device=dev), transposed=not nk,
+                                                 out_dtype=torch.float32)
+        want, = torch.autograd.grad((y * dyv).sum(), x)
+        within(got, want, mm_tol(want, mag, N, torch.float32), f"{counts}")
+
+
 GROUPS = {
     "even": [40, 40, 40, 40], "ragged": [1, 0, 129, 77, 0, 3, 256, 128, 5], "one": [0, 0, 300, 0], "none": [0, 0, 0], "behind": [10, 20, 0],
     "many": [i % 5 for i in range(67)], "single": [1] * 40, "large": [700, 3, 513], "most": [3 if i % 7 == 0 else 0 for i in range(1024)],
@@ -647,6 +674,56 @@ def test_results_repeat_bit_for_bit(pkg, dev):
     g0 = pkg.moe_token_unpermute_grad(dout, L.y, L.place, L.probs)
     for _ in range(3):
         assert all(torch.equal(u, v) for u, v in zip(g0, pkg.moe_token_unpermute_grad(dout, L.y, L.place, L.probs)))
+
+
+def test_offsets_beyond_32_bits(pkg, dev):
+    """More than 2^32 bytes, and more than 2^31 elements, behind every tensor that can be so long: the last rows are right."""
+    def random_codes(*shape):
+        q = torch.empty(shape, dtype=torch.uint8, device=dev)
+        q.random_(0, 120)                                   # no NaN codes
+        return q.view(F8)
+
+    D, rows = 4096, (1 << 19) + 1029                        # quantiser, on 2^31 and more elements
+    x = torch.zeros((rows, D), dtype=torch.bfloat16, device=dev)
+    last = activations(gen(31), (3, D), torch.bfloat16)
+    x[-3:] = last.to(dev)
+    q, s = pkg.block_quant_fp8(x)
+    rq, rs = quant_ref(last, F8)
+    assert torch.equal(s[-3:].cpu(), rs) and torch.equal(q[-3:].view(torch.uint8).cpu(), rq)
+    # the same rows sorted, all but the last behind one expert, and summed again
+    ids = torch.zeros((rows, 1), dtype=torch.int32, device=dev)
+    ids[-2] = 1
+    r, place, counts = pkg.moe_token_permute(x, ids, 3)
+    assert counts.tolist() == [rows - 1, 1, 0] and place[-3:, 0].tolist() == [rows - 3, rows - 1, rows - 2]
+    assert torch.equal(r[-3:], x[[-3, -1, -2]])
+    assert torch.equal(pkg.moe_token_unpermute(r, place)[-3:], x[-3:])
+    assert torch.equal(pkg.moe_token_permute_grad(r, place)[-3:], x[-3:])
+    probs = torch.full((rows, 1), 0.5, device=dev)
+    dr, dp = pkg.moe_token_unpermute_grad(x, r, place, probs, out=torch.empty_like(x))
+    assert torch.equal(dr[-3:], 0.5 * x[[-3, -1, -2]])
+    sq = (last.double() ** 2).sum(1, keepdim=True)
+    within(dp[-3:], sq, sq * D * 2.0 ** -23)
+    del x, q, s, r, dr, ids, place
+    M, N, K = 70003, 32768, 144                             # product: the output, for many and for few rows
+    xq, wq = random_codes(M, K), random_codes(N, K)
+    xs, ws = torch.rand((M, 2), device=dev), torch.rand((N // 128, 2), device=dev)
+    out = pkg.block_quant_matmul(xq, xs, wq, ws, transposed=True)
+    want, mag = mm_ref(xq[-2:].cpu(), xs[-2:].cpu(), wq.cpu(), ws.cpu(), True)
+    within(out[-2:], want, mm_tol(want, mag, K, torch.bfloat16))
+    del out, wq
+    E, K, N = 1024, 2048, 2064                              # and the experts' weights
+    for nk in (True, False):
+        w = random_codes(E, N, K) if nk else random_codes(E, K, N)
+        ws = torch.rand((E, 17, 16) if nk else (E, 16, 17), device=dev)
+        for M in (9, 400):
+            xq, xs = random_codes(M, K), torch.rand((M, 16), device=dev)
+            counts = torch.zeros(E, dtype=torch.int64, device=dev)
+            counts[-1], counts[3] = M - 2, 2
+            out = pkg.block_quant_grouped_matmul(xq, xs, w, ws, counts, transposed=nk)
+            for lo, hi, e in ((0, 2, 3), (2, M, E - 1)):
+                want, mag = mm_ref(xq[lo:hi].cpu(), xs[lo:hi].cpu(), w[e].cpu(), ws[e].cpu(), nk)
+                within(out[lo:hi], want, mm_tol(want, mag, K, torch.bfloat16), f"{nk} {M} {e}")
+        del w
 
 
 def test_refusals_on_the_device(pkg, dev):

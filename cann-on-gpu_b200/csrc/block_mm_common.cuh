@@ -124,28 +124,40 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t local, uint32_t cta)
     asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
     return v;
 }
-// Four sums of a row to columns n .. n + 3 of out (element `at` is column n; n a multiple of 4).
-__device__ __forceinline__ void store_quad(const BmParams &p, int64_t at, int n, const float4 &v) {
-    if (p.vec_out && n < p.N) {                           // N a multiple of 8, 16-byte aligned
-        if (p.out_type == ET_F32) {
-            *reinterpret_cast<float4 *>((float *)p.out + at) = v;
+// Four sums of a row to out[at ..], of which `left` columns lie inside the row; vec: N a multiple of 8, 16-byte aligned.  The
+// type is a template argument: code that a launch runs once comes from memory, and a branch on the type at every store made
+// the end of a tile of 64 rows 5 us longer.
+template <int T>
+__device__ __forceinline__ void store_quad(void *out, bool vec, int64_t at, int left, const float4 &v) {
+    if constexpr (T == ET_F32) {
+        float *o = (float *)out + at;
+        if (vec) {
+            if (left > 0) *reinterpret_cast<float4 *>(o) = v;
         } else {
-            uint2 w;
-            if (p.out_type == ET_BF16) {
-                __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
-                w = make_uint2(*reinterpret_cast<uint32_t *>(&a), *reinterpret_cast<uint32_t *>(&b));
-            } else {
-                __half2 a = __floats2half2_rn(v.x, v.y), b = __floats2half2_rn(v.z, v.w);
-                w = make_uint2(*reinterpret_cast<uint32_t *>(&a), *reinterpret_cast<uint32_t *>(&b));
-            }
-            *reinterpret_cast<uint2 *>((uint16_t *)p.out + at) = w;
+            if (left > 0) o[0] = v.x;
+            if (left > 1) o[1] = v.y;
+            if (left > 2) o[2] = v.z;
+            if (left > 3) o[3] = v.w;
         }
-        return;
+    } else {
+        uint16_t *o = (uint16_t *)out + at;
+        uint2 w;
+        if constexpr (T == ET_BF16) {
+            __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
+            w = make_uint2(*reinterpret_cast<uint32_t *>(&a), *reinterpret_cast<uint32_t *>(&b));
+        } else {
+            __half2 a = __floats2half2_rn(v.x, v.y), b = __floats2half2_rn(v.z, v.w);
+            w = make_uint2(*reinterpret_cast<uint32_t *>(&a), *reinterpret_cast<uint32_t *>(&b));
+        }
+        if (vec) {
+            if (left > 0) *reinterpret_cast<uint2 *>(o) = w;
+        } else {
+            if (left > 0) o[0] = (uint16_t)w.x;
+            if (left > 1) o[1] = (uint16_t)(w.x >> 16);
+            if (left > 2) o[2] = (uint16_t)w.y;
+            if (left > 3) o[3] = (uint16_t)(w.y >> 16);
+        }
     }
-    if (n < p.N) store_from_float(p.out, p.out_type, at, v.x);
-    if (n + 1 < p.N) store_from_float(p.out, p.out_type, at + 1, v.y);
-    if (n + 2 < p.N) store_from_float(p.out, p.out_type, at + 2, v.z);
-    if (n + 3 < p.N) store_from_float(p.out, p.out_type, at + 3, v.w);
 }
 
 // The table of a launch, filled by one warp: rows of expert e are row_start[e] .. row_start[e + 1], its tiles end at

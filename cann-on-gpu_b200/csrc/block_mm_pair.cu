@@ -99,31 +99,34 @@ __device__ __forceinline__ void store_rows(const uint64_t (&acc)[64], uint4 *box
     }
 }
 
-// Sums of SPLIT pairs, in order: this pair's share of the columns, 4 a lane, all of a lane's reads in flight at once.
-template <int SPLIT>
+// Sums of SPLIT pairs, in order: this pair's share of the columns, 4 a lane, the reads of some rows in flight at once.
+template <int SPLIT, int T>
 __device__ __forceinline__ void join_pairs(const BmParams &p, uint32_t sums, uint32_t pitch, int crank, int ew, int m0, int rows, int n0) {
-    constexpr int SHARE = BP_COLS / SPLIT, PER_ROW = SHARE / 4, AT_ONCE = 32 / PER_ROW, ROWS = 128 / (BP_EPI * AT_ONCE);
-    const int lane = threadIdx.x & 31, col = (crank >> 1) * SHARE + (lane % PER_ROW) * 4, n = n0 + col, r0 = ew * AT_ONCE + lane / PER_ROW;
-    float4 v[SPLIT][ROWS];
+    constexpr int SHARE = BP_COLS / SPLIT, PER_ROW = SHARE / 4, AT_ONCE = 32 / PER_ROW, STEP = BP_EPI * AT_ONCE, FLIGHT = 16 / SPLIT;
+    const int lane = threadIdx.x & 31, col = (crank >> 1) * SHARE + (lane % PER_ROW) * 4, n = n0 + col;
+    uint32_t from[SPLIT];
 #pragma unroll
-    for (int j = 0; j < SPLIT; ++j) {
-        const uint32_t from = bp_at(sums + (uint32_t)col * 4u, (uint32_t)(2 * j + (crank & 1)));
+    for (int j = 0; j < SPLIT; ++j) from[j] = bp_at(sums + (uint32_t)col * 4u, (uint32_t)(2 * j + (crank & 1)));
+#pragma unroll 1
+    for (int r0 = ew * AT_ONCE + lane / PER_ROW; r0 < rows && r0 < 128; r0 += STEP * FLIGHT) {
+        float4 v[SPLIT][FLIGHT];
 #pragma unroll
-        for (int u = 0; u < ROWS; ++u) {
-            const int r = r0 + u * BP_EPI * AT_ONCE;
-            v[j][u] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (r < rows)
-                asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                             : "=f"(v[j][u].x), "=f"(v[j][u].y), "=f"(v[j][u].z), "=f"(v[j][u].w) : "r"(from + (uint32_t)r * pitch) : "memory");
+        for (int j = 0; j < SPLIT; ++j)
+#pragma unroll
+            for (int u = 0; u < FLIGHT; ++u) {
+                v[j][u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (r0 + u * STEP < 128)
+                    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                 : "=f"(v[j][u].x), "=f"(v[j][u].y), "=f"(v[j][u].z), "=f"(v[j][u].w) : "r"(from[j] + (uint32_t)(r0 + u * STEP) * pitch) : "memory");
+            }
+#pragma unroll
+        for (int u = 0; u < FLIGHT; ++u) {
+            const int r = r0 + u * STEP;
+            float4 t = v[0][u];
+#pragma unroll
+            for (int j = 1; j < SPLIT; ++j) { t.x += v[j][u].x; t.y += v[j][u].y; t.z += v[j][u].z; t.w += v[j][u].w; }
+            if (r < rows && r < 128) store_quad<T>(p.out, p.vec_out, (int64_t)(m0 + r) * p.N + n, p.N - n, t);
         }
-    }
-#pragma unroll
-    for (int u = 0; u < ROWS; ++u) {
-        const int r = r0 + u * BP_EPI * AT_ONCE;
-        float4 t = v[0][u];
-#pragma unroll
-        for (int j = 1; j < SPLIT; ++j) { t.x += v[j][u].x; t.y += v[j][u].y; t.z += v[j][u].z; t.w += v[j][u].w; }
-        if (r < rows) store_quad(p, (int64_t)(m0 + r) * p.N + n, n, t);
     }
 }
 
@@ -367,8 +370,11 @@ block_mm_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
             walk.seek(first, e, m0, rows, n0);
             m0 += rank * 128;
             rows -= rank * 128;
-            if (p.split == 2) join_pairs<2>(p, base, PITCH, crank, ew, m0, rows, n0);
-            else join_pairs<4>(p, base, PITCH, crank, ew, m0, rows, n0);
+#define JOIN(T) (p.split == 2 ? join_pairs<2, T>(p, base, PITCH, crank, ew, m0, rows, n0) : join_pairs<4, T>(p, base, PITCH, crank, ew, m0, rows, n0))
+            if (p.out_type == ET_BF16) JOIN(ET_BF16);
+            else if (p.out_type == ET_F16) JOIN(ET_F16);
+            else JOIN(ET_F32);
+#undef JOIN
             bm_cluster_sync();                            // a CTA's shared memory outlives the others' reads
         }
     }

@@ -50,6 +50,28 @@ __device__ __forceinline__ void bm_mma(uint32_t d_tmem, uint64_t a_desc, uint64_
         "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
         ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
 }
+// The first `rows` of a thread's sums to one column of out.
+template <int T, int PAIRS, typename E>
+__device__ __forceinline__ void store_column(const uint64_t (&acc)[PAIRS], E *o, int rows, int N) {
+#pragma unroll
+    for (int i = 0; i < 2 * PAIRS; i += 2) {
+        float f0, f1;
+        E e0, e1;
+        unpack2(acc[i / 2], f0, f1);
+        if constexpr (T == ET_F32) {
+            e0 = f0; e1 = f1;
+        } else {
+            uint32_t h;
+            if constexpr (T == ET_BF16) { __nv_bfloat162 b = __floats2bfloat162_rn(f0, f1); h = *reinterpret_cast<uint32_t *>(&b); }
+            else { __half2 b = __floats2half2_rn(f0, f1); h = *reinterpret_cast<uint32_t *>(&b); }
+            e0 = (E)h; e1 = (E)(h >> 16);
+        }
+        if (i < rows) *o = e0;
+        o += N;
+        if (i + 1 < rows) *o = e1;
+        o += N;
+    }
+}
 template <int NT>
 __global__ void __launch_bounds__(BT_THREADS, 1)
 block_mm_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w, const BmParams p, const uint32_t idesc) {
@@ -255,15 +277,12 @@ block_mm_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
             } else {
                 int e, m0, rows, n0;
                 walk.seek(tile, e, m0, rows, n0);
-                const int n = n0 + ln;
+                const int n = n0 + ln, r0 = set * S::COLS;
                 if (n < p.N) {
-#pragma unroll
-                    for (int i = 0; i < S::COLS; ++i) {
-                        float f0, f1;
-                        unpack2(acc[i / 2], f0, f1);
-                        const int r = set * S::COLS + i;
-                        if (r < rows) store_from_float(p.out, p.out_type, (int64_t)(m0 + r) * p.N + n, (i & 1) ? f1 : f0);
-                    }
+                    const int64_t at = (int64_t)(m0 + r0) * p.N + n;
+                    if (p.out_type == ET_BF16) store_column<ET_BF16>(acc, (uint16_t *)p.out + at, rows - r0, p.N);
+                    else if (p.out_type == ET_F16) store_column<ET_F16>(acc, (uint16_t *)p.out + at, rows - r0, p.N);
+                    else store_column<ET_F32>(acc, (float *)p.out + at, rows - r0, p.N);
                 }
                 __syncwarp();
             }
@@ -287,7 +306,10 @@ block_mm_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
                 for (int c = 1; c < 8; ++c)
                     if (c < p.split) { v.x += part[c].x; v.y += part[c].y; v.z += part[c].z; v.w += part[c].w; }
                 const int n = n0 + lane * 4;
-                store_quad(p, (int64_t)(m0 + r) * p.N + n, n, v);
+                const int64_t at = (int64_t)(m0 + r) * p.N + n;
+                if (p.out_type == ET_BF16) store_quad<ET_BF16>(p.out, p.vec_out, at, p.N - n, v);
+                else if (p.out_type == ET_F16) store_quad<ET_F16>(p.out, p.vec_out, at, p.N - n, v);
+                else store_quad<ET_F32>(p.out, p.vec_out, at, p.N - n, v);
             }
         }
         bm_cluster_sync();                                // a CTA's shared memory outlives the others' reads
@@ -341,39 +363,44 @@ bool block_mm_tc_supported(const BlockMmArgs &a) {
     return (a.M / 16 + a.experts + 1) * ((a.N + 127) / 128) < (1LL << 30);
 }
 
-// The form with the least estimated time.  Rounds of tiles over the SMs x the measured time of a step of K: 0.62, 0.78
-// and 1.0 us per group of two blocks with 16, 32 and 64 rows a tile (1 us more where a cluster cuts K), 0.42 us per block and pair
-// of CTAs with 256 x 256 tiles (6 or 9 us more for a K cut by 2 or 4: the meeting, 128 KB of sums written and read back).
-// Microseconds, this form / pairs / pairs with K cut by 2: 64 x 4096 x 14336 18.7 / 18.8 / -, 128 x 4096 x 14336 29.9 / 19.8 / -,
-// 128 x 4096 x 4096 11.8 / 16.9 / 16.6, 77 x 4112 x 2000 9.7 / 17 / -, 256 x 14336 x 4096 - / 44.8 / 31.3; 64 experts, 2048 x 2816, 16 rows
-// each 64 / 81, 32 rows 84 / 88, 64 rows 126 / 91.  A form with 128 rows a tile was never the fastest.
+// The form with the least estimated time (us): a fixed part, and the longer of two, the weights from HBM or the rounds of tiles
+// over the SMs, with some of the shorter.  A round is the measured time of a step of K -- 0.36, 0.40 and 0.50 per group of two
+// blocks with 16, 32 and 64 rows a tile, 0.41 per block and pair of CTAs with 256 x 256 tiles -- and of a tile's stores.
+// Measured with 16 / 32 / 64 rows a tile / pairs: 64 x 4096 x 14336 27.7 / 17.8 / 14.5 / 19.0, 128 x 4096 x 14336 - / 29.2 / 20.7 / 19.8,
+// 256 x 4096 x 4096 - / - / 12.2 / 17.4, 64 experts of 2048 x 2816 with 4 rows each 54 / 54 / 56 / 76, with 32 rows 85 / 69 / 67 / 88, with 128
+// rows - / 157 / 120 / 110.  Tiles of 128 rows on one CTA were the fastest nowhere (21.7 and 16.9 on the second and third).
 // The rows of an expert are not known here: their mean stands in, with half a tile more per expert.
 cudaError_t launch_block_mm_tc(const BlockMmArgs &a, cudaStream_t s) {
     const int64_t nkb = (a.K + BM_BK - 1) / BM_BK, groups = (nkb + 1) / 2, sms = sm_count();
     const double experts = a.experts > 0 ? (double)std::min(a.experts, a.M) : 1.0, mean = (double)a.M / experts;
+    const double hbm = experts * (double)a.K * (double)a.N / 6.2e6;
     auto rounds = [&](int tile_rows, int tile_cols, double slots) {
         const double per = a.experts > 0 ? std::max(1.0, mean / tile_rows + 0.5) : std::ceil(mean / tile_rows);
-        return experts * per * (double)((a.N + tile_cols - 1) / tile_cols) / slots;
+        return std::ceil(experts * per * (double)((a.N + tile_cols - 1) / tile_cols) / slots);
     };
+    auto time = [&](double fixed, double sm) { return fixed + std::max(hbm, sm) + 0.15 * std::min(hbm, sm); };
     // the most tiles there can be, whatever the experts' rows: a cluster that cuts K has one tile
     auto most = [&](int tile_rows, int tile_cols) {
         const int64_t full = (a.M + tile_rows - 1) / tile_rows;
         return (a.experts > 0 ? std::min<int64_t>(a.M, full + a.experts - 1) : full) * ((a.N + tile_cols - 1) / tile_cols);
     };
+    // clusters of 2, 4 and 8 CTAs, one CTA per SM, that run at once: 74, 33 and 15 with 148 SMs (none crosses a GPC)
+    auto clusters = [&](int ctas) { return ctas == 1 ? sms : (ctas == 2 ? sms / 2 : (ctas == 4 ? sms * 33 / 148 : sms * 15 / 148)); };
     int best_nt = 0, best_split = 1;
-    double best = std::ceil(rounds(256, 256, (double)(sms / 2))) * (double)nkb * 0.42;
+    double best = time(6.2, rounds(256, 256, (double)(sms / 2)) * ((double)nkb * 0.41 + 1.3));
     for (int split = 2; split <= 4; split *= 2) {
-        // clusters of 4 and 8 CTAs: 33 and 15 of them fit 148 SMs at once
-        if ((double)most(256, 256) > (double)sms / (split == 2 ? 4.5 : 9.9) || split * 8 > nkb) break;
-        const double t = (double)((nkb + split - 1) / split) * 0.42 + (split == 2 ? 6.0 : 9.0);
+        if (most(256, 256) > clusters(2 * split) || split * 8 > nkb) break;
+        const double t = time(split == 2 ? 7.2 : 9.2, (double)((nkb + split - 1) / split) * 0.41 + 1.3);
         if (t < best) { best = t; best_split = split; }
     }
     const int nts[3] = {16, 32, 64};
-    const double step_us[3] = {0.62, 0.78, 1.0};
+    const double step_us[3] = {0.36, 0.40, 0.50};
     for (int i = 0; i < 3; ++i) {
         int split = 1;
-        while (split < 8 && most(nts[i], BM_LANES) * split * 2 <= sms && split * 4 <= groups) split *= 2;
-        const double t = std::ceil(rounds(nts[i], BM_LANES, (double)sms) * split) * (double)((groups + split - 1) / split) * step_us[i] + (split > 1 ? 1.0 : 0.0);
+        while (split < 8 && most(nts[i], BM_LANES) <= clusters(2 * split) && split * 4 <= groups) split *= 2;
+        // (where K is cut all tiles run at once)
+        const double r = split > 1 ? 1.0 : rounds(nts[i], BM_LANES, (double)sms);
+        const double t = time(split > 1 ? 7.0 : 5.5, r * ((double)((groups + split - 1) / split) * step_us[i] + 0.4));
         if (t < best) { best = t; best_nt = nts[i]; best_split = split; }
     }
     switch (best_nt) {

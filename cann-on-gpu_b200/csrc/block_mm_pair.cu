@@ -415,9 +415,7 @@ cudaError_t launch_block_mm_pair(const BlockMmArgs &a, int split, cudaStream_t s
     cudaError_t e = allow_smem<block_mm_pair_kernel>(BpSmem::TOTAL);
     if (e != cudaSuccess) return e;
     if (!has_regs<block_mm_pair_kernel>(168)) return cudaErrorInvalidConfiguration;
-    e = launch_chained(block_mm_pair_kernel, (unsigned)(2 * pairs), BP_THREADS, BpSmem::TOTAL, (unsigned)(2 * split), s, tx, tw, p, idesc);
-    if (e == cudaSuccess) count_launch();
-    return e;
+    return launch_chained(block_mm_pair_kernel, (unsigned)(2 * pairs), BP_THREADS, BpSmem::TOTAL, (unsigned)(2 * split), s, tx, tw, p, idesc);
 }
 
 unsigned int block_mm_pair_device_status() {

@@ -350,9 +350,7 @@ template <int NT> cudaError_t launch_form(const BlockMmArgs &a, int split, cudaS
     cudaError_t e = allow_smem<block_mm_tc_kernel<NT>>(S::TOTAL);
     if (e != cudaSuccess) return e;
     if (!has_regs<block_mm_tc_kernel<NT>>(168)) return cudaErrorInvalidConfiguration;
-    e = launch_chained(block_mm_tc_kernel<NT>, (unsigned)grid, BT_THREADS, S::TOTAL, (unsigned)split, s, tx, tw, p, idesc);
-    if (e == cudaSuccess) count_launch();
-    return e;
+    return launch_chained(block_mm_tc_kernel<NT>, (unsigned)grid, BT_THREADS, S::TOTAL, (unsigned)split, s, tx, tw, p, idesc);
 }
 
 }  // namespace

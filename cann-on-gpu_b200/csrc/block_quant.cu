@@ -14,6 +14,7 @@
 // block and share its maximum by three or four shuffles; with 8 values a lane the two divisions per block and the
 // addresses were done twice as often (4099 x 14336 bf16: 39.7 us).
 #include "device_utils.cuh"
+#include "launch_utils.h"
 
 namespace qmm {
 namespace {
@@ -71,6 +72,8 @@ template <int T, int N, int STEP> __device__ __forceinline__ void load_each(cons
 template <int T, int N, bool VEC, bool SWIGLU, bool E5M2>
 __global__ void __launch_bounds__(256) block_quant_kernel(const void *x, uint8_t *q, float *scale_out, uint32_t nblocks, uint32_t kb, int64_t D) {
     constexpr int LPB = 128 / N;                          // lanes of a block
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const uint32_t b = blockIdx.x * (256u / LPB) + threadIdx.x / LPB, r = b / kb;
     const int c0 = (threadIdx.x % LPB) * (VEC ? N : 1);
     const int64_t col = (int64_t)(b - r * kb) * 128 + c0, rest = D - col, at = (int64_t)r * D + col;
@@ -124,6 +127,8 @@ __global__ void __launch_bounds__(256) block_quant_kernel(const void *x, uint8_t
 template <int T, bool VEC, bool E5M2>
 __global__ void __launch_bounds__(256) tile_quant_kernel(const void *x, uint8_t *q, float *scale_out, int64_t rows, uint32_t kb, int64_t D) {
     __shared__ float sh[8];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const int64_t r0 = (int64_t)(blockIdx.x / kb) * 128, col = (int64_t)(blockIdx.x % kb) * 128 + (threadIdx.x & 15) * 8;
     const int64_t rest = D - col;
     float f[8][8], m = 0.f;
@@ -168,10 +173,8 @@ cudaError_t launch_rows(const void *x, bool swiglu, uint8_t *q, float *scale_out
     if (n > 0x7fffffffLL) return cudaErrorInvalidValue;
     constexpr int PER_CTA = 256 / (128 / N);
     const unsigned g = (unsigned)((n + PER_CTA - 1) / PER_CTA);
-    if (swiglu) block_quant_kernel<T, N, VEC, true, E5M2><<<g, 256, 0, s>>>(x, q, scale_out, (uint32_t)n, (uint32_t)kb, D);
-    else block_quant_kernel<T, N, VEC, false, E5M2><<<g, 256, 0, s>>>(x, q, scale_out, (uint32_t)n, (uint32_t)kb, D);
-    count_launch();
-    return cudaGetLastError();
+    return launch_chained(swiglu ? block_quant_kernel<T, N, VEC, true, E5M2> : block_quant_kernel<T, N, VEC, false, E5M2>, g, 256, 0, 1, s, x, q, scale_out,
+                          (uint32_t)n, (uint32_t)kb, D);
 }
 template <int T, bool E5M2>
 cudaError_t launch_typed(const void *x, int64_t row_block, bool swiglu, uint8_t *q, float *scale_out, int64_t rows, int64_t D, cudaStream_t s) {
@@ -179,10 +182,8 @@ cudaError_t launch_typed(const void *x, int64_t row_block, bool swiglu, uint8_t 
     if (row_block == 128) {
         const int64_t kb = (D + 127) / 128, n = (rows + 127) / 128 * kb;
         if (n > 0x7fffffffLL) return cudaErrorInvalidValue;
-        if (D % 8 == 0 && ax % 16 == 0) tile_quant_kernel<T, true, E5M2><<<(unsigned)n, 256, 0, s>>>(x, q, scale_out, rows, (uint32_t)kb, D);
-        else tile_quant_kernel<T, false, E5M2><<<(unsigned)n, 256, 0, s>>>(x, q, scale_out, rows, (uint32_t)kb, D);
-        count_launch();
-        return cudaGetLastError();
+        return launch_chained(D % 8 == 0 && ax % 16 == 0 ? tile_quant_kernel<T, true, E5M2> : tile_quant_kernel<T, false, E5M2>, (unsigned)n, 256, 0, 1, s, x, q,
+                              scale_out, rows, (uint32_t)kb, D);
     }
     if constexpr (T == ET_F32) {
         if (D % 8 == 0 && ax % 32 == 0 && aq % 8 == 0) return launch_rows<T, 8, true, E5M2>(x, swiglu, q, scale_out, rows, D, s);

@@ -45,8 +45,9 @@ template <auto Kernel> bool has_regs(int regs) {
     }
     return n == regs;
 }
-// Launch that may start while the kernel before it on the stream drains (the kernel waits with griddepcontrol.wait
-// before it touches global memory), as clusters of `cluster` CTAs.
+// Launch that may start while the kernel before it on the stream drains, as clusters of `cluster` CTAs.  Such a kernel
+// waits with griddepcontrol.wait before it touches global memory, and lets its own successor start with
+// griddepcontrol.launch_dependents: what a launch costs besides its work (some 2 us) then passes beside the kernel before it.
 template <typename... P, typename... A>
 cudaError_t launch_chained(void (*kernel)(P...), unsigned grid, unsigned threads, size_t smem, unsigned cluster, cudaStream_t s, A... args) {
     cudaLaunchConfig_t cfg{};
@@ -63,24 +64,6 @@ cudaError_t launch_chained(void (*kernel)(P...), unsigned grid, unsigned threads
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = cluster > 1 ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
-}
-
-// Launch of clusters of `cluster` CTAs, behind everything before it on the stream.
-template <typename... P, typename... A>
-cudaError_t launch_cluster(void (*kernel)(P...), unsigned grid, unsigned threads, size_t smem, unsigned cluster, cudaStream_t s, A... args) {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = cluster;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
     if (cluster > 8) {
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e != cudaSuccess) return e;
@@ -89,6 +72,7 @@ cudaError_t launch_cluster(void (*kernel)(P...), unsigned grid, unsigned threads
     if (e == cudaSuccess) count_launch();
     return e;
 }
+
 // Whether the current device can hold such a cluster of `Kernel` at all.
 template <auto Kernel> bool cluster_fits(unsigned cluster, unsigned threads, size_t smem) {
     static std::atomic<int> known[64];   // 0 unknown, 1 no, 2 yes
@@ -128,9 +112,7 @@ template <auto Kernel, typename... A> cudaError_t launch_resident(int64_t work, 
         if (slot < 8) known[dev][slot].store(per_sm, std::memory_order_relaxed);
     }
     const int64_t most = (int64_t)per_sm * sm_count();
-    Kernel<<<(unsigned)(work < most ? work : most), threads, 0, s>>>(args...);
-    count_launch();
-    return cudaGetLastError();
+    return launch_chained(Kernel, (unsigned)(work < most ? work : most), (unsigned)threads, 0, 1, s, args...);
 }
 
 }  // namespace qmm

@@ -60,6 +60,8 @@ moe_sort_kernel(const void *ids, bool ids64, int32_t *place, int64_t *counts, in
     const int64_t share = (N + SORT_CTAS * SORT_WARPS * 32 - 1) / (SORT_CTAS * SORT_WARPS * 32) * 32;
     const int64_t lo = (int64_t)(cta * SORT_WARPS + warp) * share, hi = lo + share < N ? lo + share : N;
     const bool kept = share <= 32 * SORT_RUN;     // one run: pass 2 finds everything in registers
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    // not before the wait: the copy kernel behind this one loads tokens at once, which the kernels before this one may have written
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     int e[SORT_RUN], at[SORT_RUN];                // expert, and the place among the warp's of that expert
     auto load = [&](int64_t i0) {
@@ -147,13 +149,14 @@ __global__ void __launch_bounds__(256) moe_scatter_kernel(const U *tokens, const
     const int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
     const int64_t t = w / segs, seg = w - t * segs;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (t >= T) return;
     U v[4];
     const int64_t u0 = seg * 128 + lane;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
         if (u0 + 32 * i < units) v[i] = __ldg(tokens + t * units + u0 + 32 * i);
-    // launched while the sort runs: the tokens are the caller's, ready before it, but the places and the rows are not
+    // launched while the sort runs: what came before the sort is complete, so the tokens are there, but the places and the rows are not
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int32_t p0 = lane < k ? place[t * k + lane] : -1, p1 = lane + 32 < k ? place[t * k + lane + 32] : -1;
     for (int j = 0; j < k; ++j) {
@@ -186,6 +189,8 @@ __global__ void __launch_bounds__(256) moe_small_permute_kernel(const void *ids,
     __shared__ int hist[MOE_MAX_EXPERTS];
     __shared__ int at[MOE_MAX_TOPK];
     const int N = T * k, t = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     U first{};
     if (t < T && tid < units) first = __ldg(tokens + (int64_t)t * units + tid);
     for (int i = tid; i < N; i += 256) {
@@ -297,6 +302,8 @@ template <int T, int B, int J>
 __global__ void __launch_bounds__(256) moe_gather_kernel(const char *rows, const int32_t *place, const void *probs, int probs_type, char *out,
                                                          int64_t n_tokens, int k, int64_t R, uint32_t pitch, int segs) {
     constexpr int W = B / 4, PAIRS = T == ET_F32 ? W / 2 : W;     // words of a lane's piece, pairs of values
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const int lane = threadIdx.x & 31;
     const int64_t w0 = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), warps = (int64_t)gridDim.x * 8;
     const int64_t t_step = warps / segs;
@@ -381,6 +388,8 @@ template <int T>
 __global__ void __launch_bounds__(256) moe_gather_scalar_kernel(const void *rows, const int32_t *place, const void *probs, int probs_type, void *out,
                                                                 int64_t n_tokens, int k, int64_t R, int64_t H, int segs) {
     using P = RowPiece<T, false>;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const int lane = threadIdx.x & 31;
     const int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), warps = (int64_t)gridDim.x * 8;
     for (int64_t item = w; item < n_tokens * segs; item += warps) {
@@ -406,6 +415,8 @@ template <int T, bool VEC, int J>
 __global__ void __launch_bounds__(256) moe_gather_grad_kernel(const void *dout, const void *rows, const int32_t *place, const void *probs, int probs_type,
                                                               void *drows, void *dprobs, int64_t n_tokens, int k, int64_t R, int64_t H, int segs) {
     using P = RowPiece<T, VEC>;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     __shared__ float part[2][8][J];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     int32_t next_pl = -1;
@@ -480,15 +491,13 @@ template <int BITS, int CTAS> cudaError_t launch_sort(const PermuteArgs &p, int6
     const cudaError_t e = allow_smem<moe_sort_kernel<BITS, CTAS>>((SORT_WARPS + 2) * MOE_MAX_EXPERTS * 4);
     if (e != cudaSuccess) return e;
     const size_t smem = (size_t)(SORT_WARPS + 2) * p.E * 4;
-    return launch_cluster(moe_sort_kernel<BITS, CTAS>, CTAS, SORT_WARPS * 32, smem, CTAS, s, p.ids, p.ids64, p.place, p.counts, N, (int)p.E);
+    return launch_chained(moe_sort_kernel<BITS, CTAS>, CTAS, SORT_WARPS * 32, smem, CTAS, s, p.ids, p.ids64, p.place, p.counts, N, (int)p.E);
 }
 template <typename U> cudaError_t launch_permute(const PermuteArgs &p, cudaStream_t s) {
     const int64_t units = p.row_bytes / (int64_t)sizeof(U), N = p.T * p.k;
     if (N <= SMALL_PAIRS) {
-        moe_small_permute_kernel<U><<<(unsigned)(p.T > 0 ? p.T : 1), 256, 0, s>>>(p.ids, p.ids64, (int)p.E, (const U *)p.tokens, p.scales, p.place, p.counts,
-                                                                                 (U *)p.rows, p.scales_out, (int)p.T, (int)p.k, units, p.S);
-        count_launch();
-        return cudaGetLastError();
+        return launch_chained(moe_small_permute_kernel<U>, (unsigned)(p.T > 0 ? p.T : 1), 256, 0, 1, s, p.ids, p.ids64, (int)p.E, (const U *)p.tokens, p.scales,
+                              p.place, p.counts, (U *)p.rows, p.scales_out, (int)p.T, (int)p.k, units, p.S);
     }
     // 16 CTAs (more than every device has to grant a cluster) where they fit: 65528 pairs over 256 experts 11.5 -> 8.5 us
     const bool wide = N > 4096 && cluster_fits<moe_sort_kernel<11, 16>>(16, SORT_WARPS * 32, (SORT_WARPS + 2) * MOE_MAX_EXPERTS * 4);
@@ -498,10 +507,8 @@ template <typename U> cudaError_t launch_permute(const PermuteArgs &p, cudaStrea
     if (e != cudaSuccess || (units == 0 && p.S == 0)) return e;
     const int64_t segs = units > 128 ? (units + 127) / 128 : 1, ctas = (p.T * segs + 7) / 8;
     if (ctas > 0x7fffffffLL) return cudaErrorInvalidValue;
-    e = launch_chained(moe_scatter_kernel<U>, (unsigned)ctas, 256, 0, 1, s, (const U *)p.tokens, p.scales, (const int32_t *)p.place, (U *)p.rows, p.scales_out,
-                       p.T, (int)p.k, units, p.S, segs);
-    if (e == cudaSuccess) count_launch();
-    return e;
+    return launch_chained(moe_scatter_kernel<U>, (unsigned)ctas, 256, 0, 1, s, (const U *)p.tokens, p.scales, (const int32_t *)p.place, (U *)p.rows, p.scales_out,
+                          p.T, (int)p.k, units, p.S, segs);
 }
 
 }  // namespace

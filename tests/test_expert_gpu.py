@@ -647,6 +647,39 @@ def test_large_permutes_captured_and_on_two_streams(pkg, dev):
         assert all(check(c, got) for c, got in zip(cases, outs))
 
 
+@pytest.mark.parametrize("dims", [(3, 2, 4, 256, 384), (40, 8, 16, 1024, 512), (700, 4, 8, 512, 512)])
+def test_layers_back_to_back(pkg, dev, dims):
+    """Kernels start while the one before them drains: layers one behind the other, whose buffers change hands between them,
+    give the bits of layers run one at a time."""
+    L = Layer(pkg, dev, *dims, seed=21, away=0.1)
+    g = gen(22)
+    xs = [torch.randn(tuple(L.x.shape), generator=g).to(device=dev, dtype=L.x.dtype) for _ in range(12)]
+    dout = [torch.randn(tuple(L.x.shape), generator=g).to(device=dev, dtype=L.x.dtype) for _ in range(12)]
+
+    def one(x, d):
+        L.x = x
+        out = L.run()
+        dy, dp = pkg.moe_token_unpermute_grad(d, L.y, L.place, L.probs)
+        return out, dp, pkg.moe_token_permute_grad(dy, L.place)
+
+    want = []
+    for x, d in zip(xs, dout):
+        torch.cuda.synchronize()
+        want.append([t.clone() for t in one(x, d)])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()                          # without the host's time between the kernels
+    with torch.cuda.graph(graph):
+        got = [one(x, d) for x, d in zip(xs, dout)]
+    for _ in range(20):
+        for outs in got:
+            for t in outs:
+                t.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert all(torch.equal(u, v) for u, v in zip(a, b))
+
+
 def test_two_streams_at_once(pkg, dev):
     """Two layers on two streams at the same time: nothing is shared between calls."""
     layers = [Layer(pkg, dev, 64, 4, 8, 512, 384, seed=5 + i) for i in range(2)]

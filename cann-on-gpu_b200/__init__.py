@@ -6,6 +6,7 @@ if the library is missing, `load()` raises.
 """
 import ctypes
 import os
+import struct
 import subprocess
 import threading
 
@@ -300,32 +301,32 @@ def cast(src, src_kind, dst_kind, n, **kw):
 
 
 # ---------------------------------------------------------------- the expert layer: fp8 with a scale per 128 (aclnn_block_quant_moe.h)
-class _Call:
-    """One operator at one set of shapes and types: its aclTensor handles and prepared phase arguments.  A handle is
-    metadata only: every call points it at its own tensors first, so nothing of a call's data is kept."""
+# aclnnB200ExpertOp
+_EXPERT_OPS = ("BlockQuantFp8", "SwiGluBlockQuantFp8", "BlockQuantMatmul", "BlockQuantGroupedMatmul", "MoeTokenPermute", "MoeTokenPermuteGrad",
+               "MoeTokenUnpermute", "MoeTokenUnpermuteGrad")
+(_OP_BLOCK_QUANT, _OP_SWIGLU_BLOCK_QUANT, _OP_BLOCK_MATMUL, _OP_GROUPED_MATMUL, _OP_PERMUTE, _OP_PERMUTE_GRAD, _OP_UNPERMUTE,
+ _OP_UNPERMUTE_GRAD) = range(8)
 
-    def __init__(self, lib, name, args):
-        import torch
-        self.lib, self.handles = lib, []
-        self.phase1, self.phase2 = getattr(lib, name + "GetWorkspaceSize"), getattr(lib, name)
-        self.set_addrs = lib.aclnnB200SetRawTensorAddrs
-        self.ws, self.ex = ctypes.c_uint64(0), ctypes.c_void_p(0)
-        self.ws_ptr, self.ws_size, self.stream = ctypes.c_void_p(0), ctypes.c_uint64(0), ctypes.c_void_p(0)
-        self.args = []
-        for a in args:
-            if isinstance(a, torch.Tensor):
+
+class _Call:
+    """One operator at one set of shapes and types: its aclTensor handles and prepared arguments.  A handle is metadata only:
+    every call points it at its own tensors first, so nothing of a call's data is kept."""
+
+    def __init__(self, lib, op, tensors, option):
+        self.lib, self.handles, self.run = lib, [], lib.aclnnB200RunExpertOp
+        n = len(tensors)
+        array = (ctypes.c_void_p * n)()
+        for i, a in enumerate(tensors):
+            if a is not None:
                 dims = (ctypes.c_int64 * max(1, a.dim()))(*a.shape)
                 h = lib.aclCreateTensor(dims, a.dim(), torch_acl_dtype(a), None, 0, ACL_FORMAT_ND, dims, a.dim(), None)
                 if not h:
                     raise RuntimeError("aclCreateTensor failed")
                 self.handles.append(h)
-                self.args.append(ctypes.c_void_p(h))
-            else:
-                self.args.append(None if a is None else (ctypes.c_bool(a) if isinstance(a, bool) else ctypes.c_int64(a)))
-        self.args += [ctypes.byref(self.ws), ctypes.byref(self.ex)]
-        n = len(self.handles)
-        self.addrs = (ctypes.c_void_p * n)()
-        self.addr_args = ((ctypes.c_void_p * n)(*self.handles), self.addrs, ctypes.c_uint64(n))
+                array[i] = h
+        self.addrs, self.stream = (ctypes.c_void_p * n)(), ctypes.c_void_p(0)
+        self.point = struct.Struct("%dQ" % n).pack_into
+        self.args = (ctypes.c_int(op), array, self.addrs, ctypes.c_uint64(n), ctypes.c_int64(option), self.stream)
 
     def __del__(self):
         try:
@@ -338,11 +339,12 @@ class _Call:
 _current_fns = None
 
 
-def _current(torch):
+def _current():
     """(current device, current stream of a device as a number): torch's own raw getters where it has them, which take a
     tenth of the public ones' time on a path whose kernels run for a few microseconds."""
     global _current_fns
     if _current_fns is None:
+        import torch
         torch.cuda.current_device()   # sets CUDA up
         raw_dev, raw_stream = getattr(torch._C, "_cuda_getDevice", None), getattr(torch._C, "_cuda_getCurrentRawStream", None)
         _current_fns = (raw_dev or torch.cuda.current_device, raw_stream or (lambda dev: torch.cuda.current_stream(dev).cuda_stream))
@@ -359,50 +361,42 @@ class _Calls(threading.local):   # a set of handles serves one call at a time: e
 _calls = _Calls()
 
 
-def _run(name, *args, stream=None, return_status=False):
-    """The two phases of `name` on torch tensors, None, integers and truth values in phase 1's order, on the tensors'
-    device and torch's current stream there (or `stream`).  A workspace, where one is needed, is the call's own."""
-    import torch
-    T = torch.Tensor
-    lib = load()
-    dev, tensors, key = None, [], [name, id(lib)]
-    for a in args:
-        if isinstance(a, T):
-            # the ABI takes dense tensors on one GPU; a view of anything else would be misread
-            i = a.get_device()
-            if i < 0 or not a.is_contiguous():
-                raise ValueError("the expert-layer operators take contiguous CUDA tensors")
-            if i != dev:
-                if dev is not None:
-                    raise ValueError(f"tensors on devices {dev} and {i}")
-                dev = i
-            tensors.append(a)
-            key.append(a.shape)
-            key.append(a.dtype)
-        else:
-            key.append(a)
-    if dev != _current(torch)[0]():
+def _run(op, tensors, option=0, stream=None, return_status=False):
+    """One operator on torch tensors (None: left out), on the tensors' device and torch's current stream there (or `stream`)."""
+    dev, key, ptrs = None, [op, option], []
+    for a in tensors:
+        if a is None:
+            key.append(None)
+            ptrs.append(0)
+            continue
+        # the ABI takes dense tensors on one GPU; a view of anything else would be misread
+        i = a.get_device()
+        if i != dev:
+            if dev is not None:
+                raise ValueError(f"tensors on devices {dev} and {i}")
+            dev = i
+        if i < 0 or not a.is_contiguous():
+            raise ValueError("the expert-layer operators take contiguous CUDA tensors")
+        key += (a.shape, a.dtype)
+        ptrs.append(a.data_ptr())
+    current_device, current_stream = _current_fns or _current()
+    if dev != current_device():
+        import torch
         with torch.cuda.device(dev):
-            return _run(name, *args, stream=stream, return_status=return_status)
-    key, known = tuple(key), _calls.known
+            return _run(op, tensors, option, stream, return_status)
+    key, known, lib = tuple(key), _calls.known, _lib or load()
     c = known.get(key)
-    if c is None:
+    if c is None or c.lib is not lib:
         if len(known) >= _calls.MOST:
             known.clear()
-        c = known[key] = _Call(lib, name, args)
-    c.addrs[:] = [t.data_ptr() for t in tensors]
-    c.set_addrs(*c.addr_args)
-    st = c.phase1(*c.args)
-    if st == ACLNN_SUCCESS:
-        need = c.ws.value
-        ws = torch.empty(need, dtype=torch.uint8, device=tensors[0].device) if need else None
-        c.ws_ptr.value, c.ws_size.value = ws.data_ptr() if need else None, need
-        c.stream.value = _current(torch)[1](dev) if stream is None else stream
-        st = c.phase2(c.ws_ptr, c.ws_size, c.ex, c.stream)
+        c = known[key] = _Call(lib, op, tensors, option)
+    c.point(c.addrs, 0, *ptrs)
+    c.stream.value = current_stream(dev) if stream is None else stream
+    st = c.run(*c.args)
     if return_status:
         return st
     if st != ACLNN_SUCCESS:
-        raise RuntimeError(f"{name} -> {st}")
+        raise RuntimeError(f"aclnnB200{_EXPERT_OPS[op]} -> {st}")
 
 
 def block_quant_fp8(x, row_block=1, dtype=None, **kw):
@@ -414,7 +408,7 @@ def block_quant_fp8(x, row_block=1, dtype=None, **kw):
     if row_block != 1:
         lead = [(x.numel() // max(D, 1) + row_block - 1) // row_block if row_block > 0 else 0]
     scale = x.new_empty((*lead, (D + 127) // 128), dtype=torch.float32)
-    _run("aclnnB200BlockQuantFp8", x, row_block, q, scale, **kw)
+    _run(_OP_BLOCK_QUANT, (x, q, scale), row_block, **kw)
     return q, scale
 
 
@@ -425,7 +419,7 @@ def swiglu_block_quant_fp8(x, dtype=None, **kw):
     D //= 2
     q = x.new_empty((*lead, D), dtype=dtype or torch.float8_e4m3fn)
     scale = x.new_empty((*lead, (D + 127) // 128), dtype=torch.float32)
-    _run("aclnnB200SwiGluBlockQuantFp8", x, q, scale, **kw)
+    _run(_OP_SWIGLU_BLOCK_QUANT, (x, q, scale), **kw)
     return q, scale
 
 
@@ -434,7 +428,7 @@ def block_quant_matmul(x, x_scale, w, w_scale, transposed=False, out_dtype=None,
     import torch
     if out is None:
         out = x.new_empty((x.shape[0], w.shape[0 if transposed else 1]), dtype=out_dtype or torch.bfloat16)
-    _run("aclnnB200BlockQuantMatmul", x, x_scale, w, w_scale, bool(transposed), out, **kw)
+    _run(_OP_BLOCK_MATMUL, (x, x_scale, w, w_scale, out), bool(transposed), **kw)
     return out
 
 
@@ -444,7 +438,7 @@ def block_quant_grouped_matmul(x, x_scale, w, w_scale, rows_per_expert, transpos
     import torch
     if out is None:
         out = x.new_empty((x.shape[0], w.shape[1 if transposed else 2]), dtype=out_dtype or torch.bfloat16)
-    _run("aclnnB200BlockQuantGroupedMatmul", x, x_scale, w, w_scale, rows_per_expert, bool(transposed), out, **kw)
+    _run(_OP_GROUPED_MATMUL, (x, x_scale, w, w_scale, rows_per_expert, out), bool(transposed), **kw)
     return out
 
 
@@ -460,21 +454,21 @@ def moe_token_permute(tokens, expert_ids, num_experts, scales=None, out=None, sc
         scales_out = scales.new_empty((out.shape[0], scales.shape[1]))
     place = tokens.new_empty((T, k), dtype=torch.int32)
     counts = tokens.new_empty((num_experts,), dtype=torch.int64)
-    _run("aclnnB200MoeTokenPermute", tokens, expert_ids, scales, out, scales_out, place, counts, **kw)
+    _run(_OP_PERMUTE, (tokens, expert_ids, scales, out, scales_out, place, counts), **kw)
     return (out, place, counts) if scales is None else (out, place, counts, scales_out)
 
 
 def moe_token_permute_grad(grad_rows, place, **kw):
     """The gradient of moe_token_permute's tokens: the sum of each token's rows of grad_rows."""
     out = grad_rows.new_empty((place.shape[0], grad_rows.shape[1]))
-    _run("aclnnB200MoeTokenPermuteGrad", grad_rows, place, out, **kw)
+    _run(_OP_PERMUTE_GRAD, (grad_rows, place, out), **kw)
     return out
 
 
 def moe_token_unpermute(rows, place, probs=None, **kw):
     """rows [R,H], place int32 [T,k], probs [T,k] -> out [T,H]: the weighted sum of each token's rows."""
     out = rows.new_empty((place.shape[0], rows.shape[1]))
-    _run("aclnnB200MoeTokenUnpermute", rows, place, probs, out, **kw)
+    _run(_OP_UNPERMUTE, (rows, place, probs, out), **kw)
     return out
 
 
@@ -485,5 +479,5 @@ def moe_token_unpermute_grad(grad_out, rows, place, probs, out=None, **kw):
     if out is None:
         out = torch.zeros_like(rows)
     dprobs = torch.empty_like(probs)
-    _run("aclnnB200MoeTokenUnpermuteGrad", grad_out, rows, place, probs, out, dprobs, **kw)
+    _run(_OP_UNPERMUTE_GRAD, (grad_out, rows, place, probs, out, dprobs), **kw)
     return out, dprobs

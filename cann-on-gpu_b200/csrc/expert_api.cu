@@ -271,12 +271,29 @@ aclnnStatus aclnnB200MoeTokenUnpermuteGradGetWorkspaceSize(const aclTensor *grad
 }
 RUN_EXPERT(aclnnB200MoeTokenUnpermuteGrad, PLAN_UNPERMUTE_GRAD)
 
-aclnnStatus aclnnB200SetRawTensorAddrs(aclTensor *const *tensors, void *const *addrs, uint64_t count) {
-    if (count > 0 && (!tensors || !addrs)) return ACLNN_ERR_PARAM_NULLPTR;
+aclnnStatus aclnnB200RunExpertOp(aclnnB200ExpertOp op, aclTensor *const *t, void *const *addrs, uint64_t count, int64_t option, aclrtStream stream) {
+    static const struct { uint64_t count; PlanOp plan; } ops[] = {
+        {3, PLAN_BLOCKQUANT}, {3, PLAN_BLOCKQUANT}, {5, PLAN_BLOCKMM}, {6, PLAN_BLOCKMM},
+        {7, PLAN_PERMUTE},    {3, PLAN_UNPERMUTE},  {4, PLAN_UNPERMUTE}, {6, PLAN_UNPERMUTE_GRAD}};
+    if ((int)op < 0 || (size_t)op >= sizeof(ops) / sizeof(ops[0])) return ACLNN_ERR_PARAM_INVALID;
+    if (!t || !addrs) return ACLNN_ERR_PARAM_NULLPTR;
+    if (count != ops[op].count) return ACLNN_ERR_PARAM_INVALID;
     for (uint64_t i = 0; i < count; ++i)
-        if (!tensors[i]) return ACLNN_ERR_PARAM_NULLPTR;
-    for (uint64_t i = 0; i < count; ++i) tensors[i]->data = addrs[i];
-    return ACLNN_SUCCESS;
+        if (t[i]) t[i]->data = addrs[i];
+    uint64_t ws = 0;
+    aclOpExecutor *e = nullptr;
+    aclnnStatus st = ACLNN_ERR_PARAM_INVALID;
+    switch (op) {
+        case ACL_B200_BLOCK_QUANT_FP8: st = block_quant_plan(t[0], option, false, t[1], t[2], &ws, &e); break;
+        case ACL_B200_SWIGLU_BLOCK_QUANT_FP8: st = block_quant_plan(t[0], 1, true, t[1], t[2], &ws, &e); break;
+        case ACL_B200_BLOCK_QUANT_MATMUL: st = block_mm_plan(t[0], t[1], t[2], t[3], nullptr, false, option != 0, t[4], &ws, &e); break;
+        case ACL_B200_BLOCK_QUANT_GROUPED_MATMUL: st = block_mm_plan(t[0], t[1], t[2], t[3], t[4], true, option != 0, t[5], &ws, &e); break;
+        case ACL_B200_MOE_TOKEN_PERMUTE: st = permute_plan(t[0], t[1], t[2], t[3], t[4], t[5], t[6], &ws, &e); break;
+        case ACL_B200_MOE_TOKEN_PERMUTE_GRAD: st = unpermute_plan(t[0], t[1], nullptr, t[2], &ws, &e); break;
+        case ACL_B200_MOE_TOKEN_UNPERMUTE: st = unpermute_plan(t[0], t[1], t[2], t[3], &ws, &e); break;
+        case ACL_B200_MOE_TOKEN_UNPERMUTE_GRAD: st = unpermute_grad_plan(t[0], t[1], t[2], t[3], t[4], t[5], &ws, &e); break;
+    }
+    return st == ACLNN_SUCCESS ? run_plan(ops[op].plan, nullptr, 0, e, stream) : st;
 }
 
 }  // extern "C"

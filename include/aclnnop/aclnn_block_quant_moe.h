@@ -106,8 +106,22 @@ ACL_FUNC_VISIBILITY aclnnStatus aclnnB200MoeTokenUnpermuteGradGetWorkspaceSize(c
     uint64_t *workspaceSize, aclOpExecutor **executor);
 B200_ACLNN_RUN(aclnnB200MoeTokenUnpermuteGrad)
 
-/* aclSetRawTensorAddr for `count` tensors in one call, for callers that keep their tensors between calls. */
-ACL_FUNC_VISIBILITY aclnnStatus aclnnB200SetRawTensorAddrs(aclTensor *const *tensors, void *const *addrs, uint64_t count);
+/* ---- Both phases in one call ---------------------------------------------------------------------
+ * For callers that keep their tensors and run an operator often: points tensors[i] at addrs[i] as aclSetRawTensorAddr does and
+ * runs the operator on the stream, with the statuses of its phases.  `tensors` are phase 1's, in its order, and as many (161002
+ * otherwise); NULL where an optional one is left out.  `option`: rowBlockSize, transposeWeight (not 0: true), else unused. */
+typedef enum {
+    ACL_B200_BLOCK_QUANT_FP8 = 0,              /* x, out, scaleOut */
+    ACL_B200_SWIGLU_BLOCK_QUANT_FP8 = 1,       /* x, out, scaleOut */
+    ACL_B200_BLOCK_QUANT_MATMUL = 2,           /* x, xScale, weight, weightScale, out */
+    ACL_B200_BLOCK_QUANT_GROUPED_MATMUL = 3,   /* x, xScale, weight, weightScale, groupRows, out */
+    ACL_B200_MOE_TOKEN_PERMUTE = 4,            /* tokens, expertIds, scales, rowsOut, scalesOut, place, rowsPerExpert */
+    ACL_B200_MOE_TOKEN_PERMUTE_GRAD = 5,       /* gradRows, place, gradTokens */
+    ACL_B200_MOE_TOKEN_UNPERMUTE = 6,          /* rows, place, probs, out */
+    ACL_B200_MOE_TOKEN_UNPERMUTE_GRAD = 7      /* gradOut, rows, place, probs, gradRows, gradProbs */
+} aclnnB200ExpertOp;
+ACL_FUNC_VISIBILITY aclnnStatus aclnnB200RunExpertOp(aclnnB200ExpertOp op, aclTensor *const *tensors, void *const *addrs, uint64_t count,
+    int64_t option, aclrtStream stream);
 
 #ifdef __cplusplus
 }

@@ -163,19 +163,32 @@ def test_phase2_refuses_before_launching(pkg):
                                                  at([1, 1], F, 0x2000), cbool(False), at([0, 32], B, 0))) == OK
 
 
-def test_set_raw_tensor_addrs(pkg):
+def test_both_phases_in_one_call(pkg):
     lib = pkg.load()
-    t = [FakeTensor(pkg, [4], pkg.ACL_FLOAT), FakeTensor(pkg, [5], pkg.ACL_FLOAT)]
+    B, F, E4 = pkg.ACL_BF16, pkg.ACL_FLOAT, pkg.ACL_FLOAT8_E4M3FN
     vp, u64 = ctypes.c_void_p, ctypes.c_uint64
-    hs, addrs = (vp * 2)(t[0].h, t[1].h), (vp * 2)(0x1000, 0x2000)
-    assert lib.aclnnB200SetRawTensorAddrs(hs, addrs, u64(2)) == OK
+
+    def run(op, tensors, addrs, option=0, count=None):
+        hs = (vp * max(1, len(tensors)))(*[t.h if t else None for t in tensors])
+        return lib.aclnnB200RunExpertOp(ctypes.c_int(op), hs, (vp * max(1, len(addrs)))(*addrs), u64(len(tensors) if count is None else count),
+                                        i64(option), vp(0))
+
+    x, q, s = FakeTensor(pkg, [4, 256], B), FakeTensor(pkg, [4, 256], E4), FakeTensor(pkg, [4, 2], F)
     got = vp(0)
-    for x, want in zip(t, (0x1000, 0x2000)):
-        assert lib.aclGetRawTensorAddr(vp(x.h), ctypes.byref(got)) == OK and got.value == want
-    assert lib.aclnnB200SetRawTensorAddrs(None, addrs, u64(2)) == NULL and lib.aclnnB200SetRawTensorAddrs(hs, None, u64(2)) == NULL
-    assert lib.aclnnB200SetRawTensorAddrs((vp * 2)(t[0].h, None), (vp * 2)(0x3000, 0), u64(2)) == NULL
-    assert lib.aclGetRawTensorAddr(vp(t[0].h), ctypes.byref(got)) == OK and got.value == 0x1000      # all or none
-    assert lib.aclnnB200SetRawTensorAddrs(None, None, u64(0)) == OK
+    assert run(0, [x, q, s], [0x10000, 0x10400, 0x30000], 1) == BAD             # codes over x
+    for t, want in ((x, 0x10000), (q, 0x10400), (s, 0x30000)):
+        assert lib.aclGetRawTensorAddr(vp(t.h), ctypes.byref(got)) == OK and got.value == want
+    assert run(0, [x, q, s], [0, 0x20000, 0x30000], 1) == NULL
+    assert run(0, [x, q, s], [0x10000, 0x20000, 0x30000], 64) == BAD            # phase 1's refusal
+    assert run(0, [x, None, s], [0x10000, 0x20000, 0x30000], 1) == NULL
+    assert run(0, [x, q, s], [0x10000, 0x20000, 0x30000], 1, count=2) == BAD
+    for op in (-1, 8, 1 << 20):
+        assert run(op, [x, q, s], [0x10000, 0x20000, 0x30000]) == BAD
+    assert lib.aclnnB200RunExpertOp(ctypes.c_int(0), None, None, u64(3), i64(1), vp(0)) == NULL
+    rows, place, out = FakeTensor(pkg, [0, 64], B), FakeTensor(pkg, [0, 2], pkg.ACL_INT32), FakeTensor(pkg, [0, 64], B)
+    assert run(5, [rows, place, out], [0, 0, 0]) == OK and run(6, [rows, place, None, out], [0, 0, 0, 0]) == OK     # empty: nothing is launched
+    w = [FakeTensor(pkg, d, t) for d, t in (([0, 64], E4), ([0, 1], F), ([64, 32], E4), ([1, 1], F), ([0, 32], B))]
+    assert run(2, w, [0, 0, 0x1000, 0x2000, 0]) == OK and run(2, w, [0, 0, 0x1000, 0x2000, 0], 1) == BAD            # [K, N], not [N, K]
 
 
 def test_wrappers_refuse_what_the_abi_would_misread(pkg):

@@ -759,6 +759,36 @@ def test_offsets_beyond_32_bits(pkg, dev):
         del w
 
 
+def test_two_phase_entries(pkg, dev):
+    """Every operator through its own two phases gives the bits of the one-call form behind the wrappers."""
+    L = Layer(pkg, dev, 20, 2, 4, 256, 384, seed=13)
+    L.run()
+    A, i64, cbool = pkg.AclTensor, ctypes.c_int64, ctypes.c_bool
+    new = lambda t: torch.zeros_like(t, dtype=torch.uint8).view(t.dtype) if t.element_size() == 1 else torch.zeros_like(t)
+    same = lambda a, b: torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+    def check(name, ins, outs, *rest):
+        got = [new(t) for t in outs]
+        pkg.call(name, *ins, *[A(t) for t in got], *rest)
+        assert all(same(a, b) for a, b in zip(got, outs)), name
+
+    q, s = new(L.q), new(L.s)
+    pkg.call("aclnnB200BlockQuantFp8", A(L.x), i64(1), A(q), A(s))
+    assert same(q, L.q) and same(s, L.s)
+    check("aclnnB200SwiGluBlockQuantFp8", [A(L.h)], [L.q2, L.s2q])
+    ids = A(L.ids)
+    rows, rs, place, counts = new(L.rows), new(L.rs), new(L.place), new(L.counts)
+    pkg.call("aclnnB200MoeTokenPermute", A(L.q), ids, A(L.s), A(rows), A(rs), A(place), A(counts))
+    assert same(rows, L.rows) and same(rs, L.rs) and same(place, L.place) and same(counts, L.counts)
+    check("aclnnB200BlockQuantGroupedMatmul", [A(L.rows), A(L.rs), A(L.w1), A(L.s1), A(L.counts), cbool(True)], [L.h])
+    one = pkg.block_quant_matmul(L.q, L.s, L.w1[0], L.s1[0], transposed=True)
+    check("aclnnB200BlockQuantMatmul", [A(L.q), A(L.s), A(L.w1[0]), A(L.s1[0]), cbool(True)], [one])
+    check("aclnnB200MoeTokenUnpermute", [A(L.y), A(L.place), A(L.probs)], [L.out])
+    check("aclnnB200MoeTokenPermuteGrad", [A(L.y), A(L.place)], [pkg.moe_token_permute_grad(L.y, L.place)])
+    dy, dp = pkg.moe_token_unpermute_grad(L.x, L.y, L.place, L.probs)
+    check("aclnnB200MoeTokenUnpermuteGrad", [A(L.x), A(L.y), A(L.place), A(L.probs)], [dy, dp])
+
+
 def test_refusals_on_the_device(pkg, dev):
     x = torch.zeros((4, 256), dtype=torch.bfloat16, device=dev)
     with pytest.raises(ValueError):

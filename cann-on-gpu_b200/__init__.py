@@ -403,10 +403,10 @@ def block_quant_fp8(x, row_block=1, dtype=None, **kw):
     """x [..., D] f32/f16/bf16 -> (fp8 codes of x's shape, fp32 scales).  One scale per 128 columns of a row
     ([..., ceil(D/128)]), or with row_block=128 per 128 x 128 block of the matrix x ([ceil(rows/128), ceil(D/128)])."""
     import torch
-    *lead, D = x.shape
+    shape = x.shape
+    D = shape[-1]
     q = torch.empty_like(x, dtype=dtype or torch.float8_e4m3fn)
-    if row_block != 1:
-        lead = [(x.numel() // max(D, 1) + row_block - 1) // row_block if row_block > 0 else 0]
+    lead = shape[:-1] if row_block == 1 else ((x.numel() // max(D, 1) + row_block - 1) // row_block if row_block > 0 else 0,)
     scale = x.new_empty((*lead, (D + 127) // 128), dtype=torch.float32)
     _run(_OP_BLOCK_QUANT, (x, q, scale), row_block, **kw)
     return q, scale
@@ -415,8 +415,8 @@ def block_quant_fp8(x, row_block=1, dtype=None, **kw):
 def swiglu_block_quant_fp8(x, dtype=None, **kw):
     """x [..., 2D] f32/f16/bf16 -> (fp8 codes [..., D] of silu(x[..., :D]) * x[..., D:], fp32 scales [..., ceil(D/128)])."""
     import torch
-    *lead, D = x.shape
-    D //= 2
+    shape = x.shape
+    lead, D = shape[:-1], shape[-1] // 2
     q = x.new_empty((*lead, D), dtype=dtype or torch.float8_e4m3fn)
     scale = x.new_empty((*lead, (D + 127) // 128), dtype=torch.float32)
     _run(_OP_SWIGLU_BLOCK_QUANT, (x, q, scale), **kw)

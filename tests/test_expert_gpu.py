@@ -187,6 +187,22 @@ def test_block_matmul_e5m2(pkg, dev, kinds, M, nk):
     within(out, want, mm_tol(want, mag, K, torch.float32))
 
 
+# rows that do not start on 16 bytes, on four, on any boundary; both types on both sides, long enough for several blocks of K
+@pytest.mark.parametrize("nk", [False, True])
+@pytest.mark.parametrize("kinds", [(F8, F8), (F8E5, F8), (F8, F8E5), (F8E5, F8E5)])
+@pytest.mark.parametrize("shape", [(70, 516, 204), (5, 519, 206), (130, 129, 67), (64, 2, 3), (200, 1027, 129)])
+def test_block_matmul_odd_rows(pkg, dev, shape, kinds, nk):
+    (M, K, N), (tx, tw) = shape, kinds
+    g = gen(M + K)
+    x, xs = codes(g, M, K, tx)
+    w, ws = quant_ref(torch.randn((N, K) if nk else (K, N), generator=g), tw, 128)
+    w = w.view(tw)
+    want, mag = mm_ref(x, xs, w, ws, nk)
+    for dtype in FLOATS:
+        out = pkg.block_quant_matmul(x.to(dev), xs.to(dev), w.to(dev), ws.to(dev), transposed=nk, out_dtype=dtype)
+        within(out, want, mm_tol(want, mag, K, dtype), f"{dtype}")
+
+
 @pytest.mark.parametrize("nk", [False, True])
 @pytest.mark.parametrize("M", [4, 96, 260])
 def test_block_matmul_tail_meets_nan_codes(pkg, dev, M, nk):

@@ -122,26 +122,26 @@ __global__ void __launch_bounds__(256) block_quant_kernel(const void *x, uint8_t
     }
 }
 
-// 128 x 128 blocks (weights, once at load time): a CTA per block, a half-warp every 16th row, the values in registers
-// between the maximum and the codes.
+// 128 x 128 blocks (weights): a CTA per block, a half-warp every 16th row, the values in registers between the maximum and the
+// codes; a lane's eight lie next to each other, or 16 apart where they are taken one by one.  8191 x 4096 bf16 20.4 us (floor 15.5).
 template <int T, bool VEC, bool E5M2>
 __global__ void __launch_bounds__(256) tile_quant_kernel(const void *x, uint8_t *q, float *scale_out, int64_t rows, uint32_t kb, int64_t D) {
     __shared__ float sh[8];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int64_t r0 = (int64_t)(blockIdx.x / kb) * 128, col = (int64_t)(blockIdx.x % kb) * 128 + (threadIdx.x & 15) * 8;
+    const int64_t r0 = (int64_t)(blockIdx.x / kb) * 128, col = (int64_t)(blockIdx.x % kb) * 128 + (threadIdx.x & 15) * (VEC ? 8 : 1);
     const int64_t rest = D - col;
     float f[8][8], m = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const int64_t r = r0 + (threadIdx.x >> 4) + 16 * i;
-        const int left = r < rows ? (int)(rest > 8 ? 8 : rest) : 0;
-        if constexpr (VEC && T != ET_F32) {
+        const int left = r < rows ? (int)(rest > 128 ? 128 : rest) : 0;
+        if constexpr (VEC) {
             Lane<T, 8> a;
             a.load(x, r * D + col, left > 0);
             a.widen(f[i]);
         } else {
-            load_each<T, 8, 1>(x, r * D + col, left, f[i]);
+            load_each<T, 8, 16>(x, r * D + col, left, f[i]);
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(f[i][j]));
@@ -157,12 +157,16 @@ __global__ void __launch_bounds__(256) tile_quant_kernel(const void *x, uint8_t 
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const int64_t r = r0 + (threadIdx.x >> 4) + 16 * i;
-        if (r >= rows) continue;
+        if (r >= rows || rest <= 0) continue;
+        uint32_t w[4];
 #pragma unroll
-        for (int j = 0; j < 8; j += 2) {
-            const uint32_t w = codes2<E5M2>(f[i][j] * inv, f[i][j + 1] * inv);
-            if (j < rest) q[r * D + col + j] = (uint8_t)w;
-            if (j + 1 < rest) q[r * D + col + j + 1] = (uint8_t)(w >> 8);
+        for (int j = 0; j < 4; ++j) w[j] = codes2<E5M2>(f[i][2 * j] * inv, f[i][2 * j + 1] * inv);
+        if constexpr (VEC) {
+            *reinterpret_cast<uint2 *>(q + r * D + col) = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (16 * j < rest) q[r * D + col + 16 * j] = (uint8_t)(w[j >> 1] >> (8 * (j & 1)));
         }
     }
 }
@@ -182,7 +186,7 @@ cudaError_t launch_typed(const void *x, int64_t row_block, bool swiglu, uint8_t 
     if (row_block == 128) {
         const int64_t kb = (D + 127) / 128, n = (rows + 127) / 128 * kb;
         if (n > 0x7fffffffLL) return cudaErrorInvalidValue;
-        return launch_chained(D % 8 == 0 && ax % 16 == 0 ? tile_quant_kernel<T, true, E5M2> : tile_quant_kernel<T, false, E5M2>, (unsigned)n, 256, 0, 1, s, x, q,
+        return launch_chained(D % 8 == 0 && ax % (T == ET_F32 ? 32 : 16) == 0 && aq % 8 == 0 ? tile_quant_kernel<T, true, E5M2> : tile_quant_kernel<T, false, E5M2>, (unsigned)n, 256, 0, 1, s, x, q,
                               scale_out, rows, (uint32_t)kb, D);
     }
     if constexpr (T == ET_F32) {
